@@ -386,6 +386,93 @@ int kvc_stage_commit(const int64_t* dst_blocks, const int64_t* dst_block_off, in
                      int64_t* staged_offsets, const int64_t* semantic, int budget, void* stream);
 
 /*
+ * Tables of one serving step from the request lengths, in one launch (no
+ * reference counterpart: there vLLM's runner builds them; the decode offsets of
+ * compressed requests that they fold in are kvc_decode_offsets above).
+ * Request r has computed[r] tokens in its semantic numbering, scheduled[r] new
+ * ones and offsets[r] tokens removed by compression (offsets NULL: none), and
+ * page_table row r (page_stride elements apart, page_width entries) names its
+ * scheduler pages of P = 128 * blocks_per_page tokens.
+ *   query_start_loc [R + 1]  prefix sums of scheduled
+ *   seq_lens [R]             computed + scheduled - offset (physical)
+ *   per token t < num_tokens of request r, j = t - query_start_loc[r]:
+ *     positions[t] = computed[r] + j (semantic, for RoPE), request_indices[t] = r,
+ *     slot_mapping[t] = page_table[r][phys / P] * P + phys % P, phys = positions[t] - offsets[r]
+ *   block_table [R][max_blocks]  128-token block ids, -1 past ceil(seq_lens[r] / 128)
+ * num_tokens is the length of the per-token arrays; entries past the step's
+ * last token get position 0, slot -1 and request -1.  computed, scheduled and
+ * page_table hold 4- or 8-byte integers (*_bytes).  A page that the table lacks
+ * (past page_width, or negative) raises KVC_DEV_BLOCK_RANGE and gives -1; a
+ * negative count, length or physical position, or more new tokens than
+ * num_tokens, raises KVC_DEV_TOKEN_RANGE; more blocks than max_blocks raise
+ * KVC_DEV_BLOCK_RANGE.  Up to 8192 requests.
+ */
+int kvc_step_tables(const void* computed, int computed_bytes, const void* scheduled, int scheduled_bytes,
+                    const int64_t* offsets, int num_requests, const void* page_table, int page_bytes,
+                    int64_t page_stride, int page_width, int blocks_per_page, int64_t num_tokens,
+                    int max_blocks, int32_t* query_start_loc, int32_t* seq_lens, int64_t* positions,
+                    int64_t* slot_mapping, int32_t* request_indices, int32_t* block_table,
+                    int32_t* error_flag, void* stream);
+
+/*
+ * Rotary positions with one or several axes (time, height, width), keys and
+ * values written into the paged cache (no reference counterpart: attention
+ * layers stay vLLM's there).  Frequency f < rotary_dim / 2 of token t turns by
+ * positions[axis_of_frequency[f]][t] * omega[f] (product and reduction in
+ * fp64), pairs (f, f + rotary_dim / 2) of each head, dims past rotary_dim pass;
+ * one rounding to the 16-bit type.  q [num_tokens][heads][head_dim] goes to
+ * q_out (which may be q with q's strides, but not overlap it otherwise), k and
+ * v [num_tokens][kv_heads][head_dim] to slot slot_mapping[t] of the caches
+ * ([num_blocks][128][kv_heads][head_dim], any block stride); a negative slot
+ * writes no key or value, one past the cache raises KVC_DEV_TOKEN_RANGE and
+ * writes none.  Of two tokens with the same slot either may stay.  All strides
+ * are in elements, multiples of 8; pointers 16-byte aligned; head_dim a
+ * multiple of 8, rotary_dim of 16 and at most 256.  axis_of_frequency may be
+ * NULL with one axis (up to 8); an entry outside [0, axes) raises
+ * KVC_DEV_INDEX_RANGE and counts as 0.
+ */
+int kvc_rotary_write(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                     int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                     int64_t v_head_stride, int dtype, int64_t num_tokens, int heads, int kv_heads,
+                     int head_dim, int rotary_dim, const int64_t* positions, int axes,
+                     int64_t position_stride, const float* omega, const int32_t* axis_of_frequency,
+                     const int64_t* slot_mapping, void* q_out, int64_t out_token_stride,
+                     int64_t out_head_stride, void* k_cache, int64_t k_block_stride, void* v_cache,
+                     int64_t v_block_stride, int64_t num_blocks, int32_t* error_flag, void* stream);
+
+/*
+ * Attention of each request's newest tokens over its paged cache, single
+ * tokens and chunks alike (no reference counterpart: attention layers stay
+ * vLLM's there).  Request r owns rows [query_start_loc[r], query_start_loc[r+1])
+ * of q and out, n of them; its cache holds seq_lens[r] physical tokens, the new
+ * ones last, in the 128-token blocks block_table[r][0..] (table_stride elements
+ * between rows, table_width entries).  New token j sits at physical position
+ * p = seq_lens[r] - n + j and sees keys i <= p and, with window > 0, of those
+ * the last `window` and the first `sinks` alone (i > p - window or i < sinks).
+ *   out = sum_i softmax_i(scale * q.k_i) v_i ; lse = log(sum_i exp(scale * q.k_i))
+ * A row that sees no key (p < 0) gets 0 and -inf.  Keys and values that a row
+ * does not see have no part in it, infinite and NaN ones included.  Rows of q
+ * that no request owns are left as they were.  lse [num_tokens][heads] may be NULL.
+ * max_query_len bounds the n; it picks the kernel, not the result.
+ * Geometries: head_dim 64, 128 or 256, heads / kv_heads <= 16, up to 8192
+ * requests.  Strides in elements, multiples of 8; pointers 16-byte aligned.
+ * workspace: kvc_paged_attention_workspace_bytes, uninitialised; a call may
+ * not share it with another that runs at the same time.  A block id outside
+ * [0, num_blocks) or past table_width raises KVC_DEV_BLOCK_RANGE and its keys
+ * count as unseen; query_start_loc entries that decrease or pass num_tokens
+ * raise KVC_DEV_INDEX_RANGE and leave that request out.
+ */
+int64_t kvc_paged_attention_workspace_bytes(int max_query_len, int heads, int kv_heads, int head_dim);
+int kvc_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype,
+                        int64_t num_tokens, int max_query_len, int heads, int kv_heads, int head_dim,
+                        const void* k_cache, int64_t k_block_stride, const void* v_cache,
+                        int64_t v_block_stride, int64_t num_blocks, const int32_t* block_table,
+                        int64_t table_stride, int table_width, const int32_t* query_start_loc,
+                        const int32_t* seq_lens, int num_requests, float scale, int window, int sinks,
+                        void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse,
+                        void* workspace, int64_t workspace_size, int32_t* error_flag, void* stream);
+
+/*
  * Tensor-parallel score sync over NVLink peer memory, replacing the MAX
  * all-reduce of the per-layer rows and the layer reduction after it (the
  * dist.all_reduce(parallel_scores, MAX) of TriAttentionMethod._select_keep_indices

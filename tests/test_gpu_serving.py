@@ -1,0 +1,402 @@
+"""Serving-step operators on the GPU against their plain 64-bit forms (tests/serving_reference.py)."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import serving_reference as R
+from vllm_ascend_kvcompress import _native as N
+from vllm_ascend_kvcompress.methods.triattention import kernels as K
+
+pytestmark = pytest.mark.gpu
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+def ints(values, dtype=torch.int32):
+    return torch.tensor(values, dtype=dtype, device="cuda")
+
+
+# ---- step tables ----------------------------------------------------------------------------------
+
+
+def check_tables(t, want):
+    got = (t.query_start_loc, t.seq_lens, t.positions, t.slot_mapping, t.request_indices, t.block_table)
+    for g, w in zip(got, want):
+        assert g.tolist() == w
+
+
+@pytest.mark.parametrize("requests,bpp,dtype,page_dtype", [
+    (1, 1, torch.int32, torch.int32), (3, 9, torch.int64, torch.int64), (300, 16, torch.int32, torch.int64),
+    (1000, 1, torch.int64, torch.int32)])
+def test_step_tables(requests, bpp, dtype, page_dtype):
+    g = torch.Generator().manual_seed(requests)
+    rand = lambda hi: torch.randint(0, hi, (requests,), generator=g).tolist()  # noqa: E731
+    computed, scheduled = rand(9000), [n if n < 40 else 0 for n in rand(60)]  # a third of them without new tokens
+    computed[0] = 0
+    offsets = [min(c, o) if o % 3 == 0 else 0 for c, o in zip(computed, rand(9000))]
+    width = -(-9100 // (128 * bpp))
+    pages = torch.randint(0, 1 << 20, (requests, width), generator=g)
+    total, blocks = sum(scheduled), 73
+    want = R.step_tables(computed, scheduled, offsets, pages.tolist(), bpp, total + 5, blocks)
+    err = ints([0])
+    t = K.step_tables(ints(computed, dtype), ints(scheduled, dtype), pages.to("cuda", page_dtype),
+                      num_tokens=total + 5, max_blocks=blocks, offsets=ints(offsets, torch.int64),
+                      blocks_per_page=bpp, error_flag=err)
+    check_tables(t, want)
+    assert err.item() == 0
+    # tables of an earlier call, and no offsets
+    want = R.step_tables(computed, scheduled, [0] * requests, pages.tolist(), bpp, total + 5, blocks)
+    again = K.step_tables(ints(computed, dtype), ints(scheduled, dtype), pages.to("cuda", page_dtype),
+                          num_tokens=total + 5, max_blocks=blocks, blocks_per_page=bpp, out=t)
+    assert again is t
+    check_tables(t, want)
+
+
+def test_step_tables_takes_rows_of_a_wider_page_table_and_an_empty_step():
+    pages = torch.arange(40, dtype=torch.int32, device="cuda").view(4, 10)[::2, 2:8]
+    t = K.step_tables(ints([130, 5]), ints([0, 0]), pages, num_tokens=0, max_blocks=3)
+    check_tables(t, ([0, 0, 0], [130, 5], [], [], [], [[2, 3, -1], [22, -1, -1]]))
+
+
+@pytest.mark.parametrize("computed,scheduled,offsets,pages,bit", [
+    ([300], [1], [0], [[4, 5]], N.DEV_BLOCK_RANGE),     # the table ends before the token's page
+    ([100], [1], [0], [[-1, 5]], N.DEV_BLOCK_RANGE),    # a page that was never assigned
+    ([10], [2], [11], [[4, 5]], N.DEV_TOKEN_RANGE),     # a token before the cache
+    ([10], [-2], [0], [[4, 5]], N.DEV_TOKEN_RANGE),     # a negative count
+    ([10], [9], [0], [[4, 5]], N.DEV_TOKEN_RANGE),      # more new tokens than the tables hold
+])
+def test_step_tables_flags_what_it_cannot_place(computed, scheduled, offsets, pages, bit):
+    err = ints([0])
+    t = K.step_tables(ints(computed), ints(scheduled), ints(pages), num_tokens=4, max_blocks=3,
+                      offsets=ints(offsets, torch.int64), error_flag=err)
+    assert err.item() & bit
+    assert all(-1 <= s < 6 * 128 for s in t.slot_mapping.tolist())
+
+
+# ---- rotary positions and cache write ---------------------------------------------------------------
+
+
+def rotary_case(n, heads, kvh, dim, rot, axes, dtype, far, seed=0, blocks=None):
+    g = torch.Generator().manual_seed(seed)
+    qkv = torch.randn(n, (heads + 2 * kvh) * dim + 8, generator=g).to(dtype)  # rows of a wider projection
+    blocks = blocks or -(-n // 128) + 1
+    return {"qkv": qkv, "split": (heads * dim, kvh * dim, kvh * dim, 8), "dim": dim,
+            "positions": torch.randint(0, far, (axes, n), generator=g),
+            "slots": torch.randperm(blocks * 128, generator=g)[:n],
+            "omega": 1e6 ** (-torch.arange(rot // 2) / (rot // 2)), "axis": (torch.arange(rot // 2) * 7 % axes).int(),
+            "kc": torch.randn(blocks, 128, kvh, dim, generator=g).to(dtype),
+            "vc": torch.randn(blocks, 128, kvh, dim, generator=g).to(dtype)}
+
+
+def views(qkv, c):
+    return [x.unflatten(1, (-1, c["dim"])) for x in qkv.split(c["split"], 1)[:3]]
+
+
+def check_rotary(c, q_got, kc_got, vc_got, slots):
+    q, k, v = views(c["qkv"], c)
+    for x, got in ((q, q_got), (k, None)):
+        want, bound = R.rotate(x, c["positions"], c["omega"], c["axis"]), R.rotate_bound(x, c["omega"], x.dtype)
+        if got is None:
+            keep = slots >= 0
+            kc, vc = c["kc"].double().flatten(0, 1), c["vc"].flatten(0, 1)
+            kb = torch.zeros_like(kc)
+            kc[slots[keep]], kb[slots[keep]] = want[keep], bound[keep]
+            vc[slots[keep]] = v[keep]
+            assert (kc_got.double().flatten(0, 1) - kc).abs().le(kb).all()
+            assert torch.equal(vc_got.flatten(0, 1), vc)
+        else:
+            assert (got.double() - want).abs().le(bound).all()
+
+
+@pytest.mark.parametrize("n,heads,kvh,dim,rot,axes,dtype,far", [
+    (1, 5, 1, 128, 128, 1, BF16, 100), (37, 16, 2, 256, 64, 3, BF16, 52000), (130, 8, 8, 64, 64, 1, FP16, 1 << 20),
+    (300, 20, 4, 128, 64, 4, FP16, 40000), (9, 3, 1, 72, 48, 2, BF16, 1 << 40), (5, 2, 2, 256, 256, 1, BF16, 7)])
+def test_rotary_write(n, heads, kvh, dim, rot, axes, dtype, far):
+    c = rotary_case(n, heads, kvh, dim, rot, axes, dtype, far)
+    if n > 4:
+        c["slots"][2] = -1  # a padded token
+    d = {k: t.cuda() for k, t in c.items() if torch.is_tensor(t)}
+    q, k, v = views(d["qkv"], c)
+    err = ints([0])
+    got = K.rotary_write(q, k, v, d["positions"][0] if axes == 1 else d["positions"], d["slots"], d["kc"], d["vc"],
+                         omega=d["omega"], axis_of_frequency=d["axis"] if axes > 1 else None, error_flag=err)
+    assert err.item() == 0
+    check_rotary(c, got.cpu(), d["kc"].cpu(), d["vc"].cpu(), c["slots"])
+    assert torch.equal(d["qkv"].cpu(), c["qkv"])  # inputs as they were
+    # in place, into caches that interleave in one padded buffer
+    both = torch.zeros(c["kc"].shape[0], 2, c["kc"][0].numel() + 64, dtype=dtype, device="cuda")
+    kc, vc = (both[:, i, : c["kc"][0].numel()].unflatten(1, c["kc"].shape[1:]) for i in (0, 1))
+    kc.copy_(c["kc"])
+    vc.copy_(c["vc"])
+    same = K.rotary_write(q, k, v, d["positions"], d["slots"], kc, vc, omega=d["omega"], axis_of_frequency=d["axis"],
+                          q_out=q)
+    assert same is q and torch.equal(q, got) and torch.equal(kc, d["kc"]) and torch.equal(vc, d["vc"])
+    assert not both[:, :, c["kc"][0].numel():].any()
+
+
+def test_rotary_write_flags_bad_slots_and_axes_and_takes_no_tokens():
+    c = rotary_case(4, 2, 1, 64, 32, 2, BF16, 50)
+    c["slots"] = torch.tensor([5, c["kc"].shape[0] * 128, -7, 1 << 40])
+    d = {k: t.cuda() for k, t in c.items() if torch.is_tensor(t)}
+    q, k, v = views(d["qkv"], c)
+    err = ints([0])
+    got = K.rotary_write(q, k, v, d["positions"], d["slots"], d["kc"], d["vc"], omega=d["omega"],
+                         axis_of_frequency=d["axis"], error_flag=err)
+    assert err.item() == N.DEV_TOKEN_RANGE
+    check_rotary(c, got.cpu(), d["kc"].cpu(), d["vc"].cpu(), torch.tensor([5, -1, -1, -1]))
+    err.zero_()
+    d["axis"][3] = 2
+    K.rotary_write(q, k, v, d["positions"], d["slots"], d["kc"], d["vc"], omega=d["omega"],
+                   axis_of_frequency=d["axis"], error_flag=err)
+    assert err.item() == N.DEV_TOKEN_RANGE | N.DEV_INDEX_RANGE
+    empty = K.rotary_write(q[:0], k[:0], v[:0], d["positions"][:, :0], d["slots"][:0], d["kc"], d["vc"],
+                           omega=d["omega"], axis_of_frequency=d["axis"])
+    assert empty.shape == (0, 2, 64)
+
+
+# ---- paged attention ------------------------------------------------------------------------------
+
+
+def attention_case(new, lens, heads, kvh, dim, dtype, seed=0, gain=1.5):
+    g = torch.Generator().manual_seed(seed)
+    need = [max(0, -(-n // 128)) for n in lens]
+    blocks = sum(need) + 3
+    ids = torch.randperm(blocks, generator=g)[: sum(need)].int()
+    table = torch.full((len(lens), max(need + [1]) + 1), -1, dtype=torch.int32)
+    at = 0
+    for r, n in enumerate(need):
+        table[r, :n] = ids[at: at + n]
+        at += n
+    starts = [0]
+    for n in new:
+        starts.append(starts[-1] + n)
+    rand = lambda *s: torch.randn(s, generator=g)  # noqa: E731
+    return {"q": (gain * rand(starts[-1], heads, dim)).to(dtype), "kc": rand(blocks, 128, kvh, dim).to(dtype),
+            "vc": rand(blocks, 128, kvh, dim).to(dtype), "table": table, "starts": starts, "lens": lens,
+            "longest": max(new)}
+
+
+def attend(c, **kw):
+    kw.setdefault("max_query_len", c["longest"])
+    return K.paged_attention(c["q"].cuda(), c["kc"].cuda(), c["vc"].cuda(), c["table"].cuda(), ints(c["starts"]),
+                             ints(c["lens"]), return_lse=True, **kw)
+
+
+def check_attention(c, got, window=0, sinks=0, scale=None):
+    scale = scale or c["q"].shape[2] ** -0.5
+    out, lse, ob, lb = R.attention(c["q"], c["kc"], c["vc"], c["table"], c["starts"], c["lens"], scale, window, sinks)
+    o, l = got[0].double().cpu(), got[1].double().cpu()
+    assert torch.equal(o.isfinite(), out.isfinite())
+    fine = out.isfinite()
+    over = ((o - out).abs() - ob)[fine]  # rows that see nothing have the bound 0
+    assert (over <= 0).all(), f"an output is {over.max().item():.3g} past its bound"
+    seen = lse > -math.inf
+    assert torch.equal(l > -math.inf, seen)
+    over = ((l - lse).abs() - lb)[seen]
+    assert (over <= 0).all(), f"an lse is {over.max().item():.3g} past its bound"
+
+
+GEOMETRIES = [(40, 8, 128, BF16), (16, 2, 256, FP16), (8, 8, 64, FP16), (5, 1, 128, BF16), (16, 1, 64, BF16),
+              (6, 2, 256, BF16), (13, 1, 128, FP16)]
+
+
+@pytest.mark.parametrize("heads,kvh,dim,dtype", GEOMETRIES)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (200, 4), (1, 0), (64, 130), (5000, 9)])
+def test_decode(heads, kvh, dim, dtype, window, sinks):
+    lens = [1, 2, 127, 128, 129, 1000, 63, 64, 65, 700]
+    c = attention_case([1] * len(lens), lens, heads, kvh, dim, dtype)
+    check_attention(c, attend(c, window=window, sinks=sinks), window, sinks)
+
+
+@pytest.mark.parametrize("heads,kvh,dim,dtype", GEOMETRIES)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (100, 4), (1, 0), (33, 300)])
+def test_short_and_ragged_chunks(heads, kvh, dim, dtype, window, sinks):
+    c = attention_case([3, 1, 0, 17, 130, 2], [3, 400, 50, 20, 300, 129], heads, kvh, dim, dtype)
+    check_attention(c, attend(c, window=window, sinks=sinks), window, sinks)
+
+
+@pytest.mark.parametrize("dim,dtype", [(128, BF16), (64, FP16), (256, BF16)])
+@pytest.mark.parametrize("new", [1, 2, 64])
+def test_one_long_request_is_cut_over_the_whole_gpu(dim, dtype, new):
+    c = attention_case([new], [9001], 4, 1, dim, dtype)
+    check_attention(c, attend(c))
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_many_requests_and_a_chunk_of_a_whole_prompt(dim):
+    new = [1] * 70 + [333] + [1] * 70
+    lens = [(37 * i) % 400 + 1 for i in range(70)] + [333] + [(91 * i) % 300 + 1 for i in range(70)]
+    c = attention_case(new, lens, 2, 1, dim, BF16)
+    check_attention(c, attend(c))
+    check_attention(c, attend(c, window=50, sinks=3), 50, 3)
+
+
+def test_rows_that_see_nothing_and_requests_without_keys():
+    c = attention_case([1, 5, 1, 3], [0, 2, 7, -4], 8, 2, 128, BF16)
+    out, lse = attend(c)
+    check_attention(c, (out, lse))
+    assert not out[:4].any() and out[4:7].any() and not out[7:].any()
+    assert (lse[:4] == -math.inf).all() and (lse[7:] == -math.inf).all()
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("dim,new", [(128, [1, 4, 30]), (64, [1, 3, 200]), (256, [2, 1, 40])])
+def test_masked_places_may_hold_anything(bad, dim, new):
+    """Slots past each request's length, keys before the window, and later new tokens."""
+    lens = [100, 300, 333]
+    c = attention_case(new, lens, 6, 2, dim, BF16)
+    for window, sinks in ((0, 0), (40, 2)):
+        d = dict(c, kc=c["kc"].clone(), vc=c["vc"].clone())
+        for r, n in enumerate(lens):
+            last = c["table"][r, (n - 1) // 128]
+            d["kc"][last, (n - 1) % 128 + 1:] = bad
+            d["vc"][last, (n - 1) % 128 + 1:] = bad
+        if window:  # a key that no row sees, in a block that rows do see
+            at = lens[1] - new[1] - window
+            d["kc"][c["table"][1, at // 128], at % 128] = bad
+            d["vc"][c["table"][1, at // 128], at % 128] = bad
+        # the last new token of the third request: its own row alone sees it
+        d["vc"][c["table"][2, (lens[2] - 1) // 128], (lens[2] - 1) % 128, 1, 5] = bad
+        out, lse = attend(d, window=window, sinks=sinks)
+        check_attention(d, (out, lse), window, sinks)
+        assert out[: sum(new) - 1].isfinite().all() and lse.isfinite().all()
+        assert (~out[-1].isfinite()).sum() == 3  # the three heads of the second KV head, one dim
+
+
+def test_infinite_and_nan_values_in_seen_places():
+    c = attention_case([2, 1], [200, 5], 4, 2, 128, BF16)
+    c["vc"][c["table"][0, 0], 17, 0, 3] = math.inf
+    c["vc"][c["table"][1, 0], 2, 1, 100] = math.nan
+    out, lse = attend(c)
+    check_attention(c, (out, lse))
+    assert (out[:2, :2, 3] == math.inf).all() and out[2, 2:, 100].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_large_scores(dtype):
+    c = attention_case([1, 40, 2], [500, 600, 20], 8, 2, 128, dtype, gain=60.0)
+    check_attention(c, attend(c))
+    check_attention(c, attend(c, scale=0.01), scale=0.01)
+
+
+@pytest.mark.parametrize("new", [[1, 2, 1], [100, 1, 60]])
+def test_strided_inputs_padded_pages_and_rows_of_no_request(new):
+    c = attention_case(new, [300, 129, 64], 10, 2, 128, BF16)
+    n = sum(new)
+    want = attend(c)
+    wide = torch.randn(n + 7, 14, 128, device="cuda").to(BF16)  # q inside a fused projection, rows behind the last
+    wide[:n, 2:12] = c["q"].cuda()
+    both = torch.full((c["kc"].shape[0], 2 * c["kc"][0].numel() + 64), math.nan, dtype=BF16, device="cuda")
+    size = c["kc"][0].numel()
+    kc, vc = (both[:, i * size: (i + 1) * size].unflatten(1, c["kc"].shape[1:]) for i in (0, 1))
+    kc.copy_(c["kc"])
+    vc.copy_(c["vc"])
+    table = torch.full((3, 9), 7, dtype=torch.int32, device="cuda")
+    table[:, : c["table"].shape[1]] = c["table"].cuda()
+    out = torch.full((n + 7, 12, 128), 3.0, dtype=BF16, device="cuda")
+    view = out[:, 1:11]
+    err = ints([0])
+    got, lse = K.paged_attention(wide[:, 2:12], kc, vc, table[:, :5], ints(c["starts"]), ints(c["lens"]),
+                                 max_query_len=c["longest"], out=view, return_lse=True, error_flag=err)
+    assert got is view and err.item() == 0
+    assert torch.equal(out[:n, 1:11], want[0]) and torch.equal(lse[:n], want[1])
+    assert (out[n:] == 3.0).all() and (out[:, 0] == 3.0).all() and (out[:, 11] == 3.0).all()
+
+
+@pytest.mark.parametrize("new", [[1, 1], [50, 1]])
+def test_bad_block_ids_and_row_ranges_are_flagged(new):
+    c = attention_case(new, [300, 100], 4, 2, 64, BF16)
+    want = attend(c)
+    err = ints([0])
+    bad = dict(c, table=c["table"].clone())
+    bad["table"][0, 1] = c["kc"].shape[0]
+    out, _ = attend(bad, error_flag=err)
+    assert err.item() == N.DEV_BLOCK_RANGE
+    assert torch.equal(out[new[0]:], want[0][new[0]:])  # the other request is served
+    err.zero_()
+    short = dict(c, table=c["table"][:, :2])
+    attend(short, error_flag=err)
+    assert err.item() == N.DEV_BLOCK_RANGE
+    err.zero_()
+    far = dict(c, starts=[0, new[0], new[0] + 9])
+    out, _ = attend(far, error_flag=err)
+    assert err.item() == N.DEV_INDEX_RANGE
+    assert torch.equal(out[: new[0]], want[0][: new[0]])
+
+
+@pytest.mark.parametrize("new", [[1] * 5, [1, 200, 3, 1, 64]])
+def test_captured_and_replayed_with_other_lengths(new):
+    lens = [300, 900, 500, 65, 64]
+    c = attention_case(new, lens, 10, 2, 128, BF16)
+    q, kc, vc, table = (c[x].cuda() for x in ("q", "kc", "vc", "table"))
+    starts, length = ints(c["starts"]), ints(lens)
+    run = lambda: K.paged_attention(q, kc, vc, table, starts, length, max_query_len=c["longest"],  # noqa: E731
+                                    return_lse=True)
+    run()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.synchronize()
+    graphs, results = [], []
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            results.append(run())
+    for shift in (0, 30):
+        c["lens"] = [n - shift for n in lens]
+        length.copy_(ints(c["lens"]))
+        for x in results:
+            x[0].zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):  # both at once: each graph has a workspace of its own
+            graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        check_attention(c, results[0])
+        assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
+
+
+def test_results_do_not_depend_on_timing():
+    c = attention_case([1, 300, 1, 2], [5000, 2300, 700, 3], 10, 2, 128, BF16)
+    d = [c[x].cuda() for x in ("q", "kc", "vc", "table")] + [ints(c["starts"]), ints(c["lens"])]
+    first = K.paged_attention(*d, max_query_len=300)
+    for _ in range(20):
+        assert torch.equal(K.paged_attention(*d, max_query_len=300), first)
+
+
+# ---- a step of all three --------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("scheduled", [[1, 1, 1, 1], [1, 70, 3, 0]])
+def test_a_step_over_a_compressed_cache(scheduled):
+    """Tables, rotary write and attention as a serving step runs them; two requests were compressed."""
+    g = torch.Generator().manual_seed(3)
+    computed, offsets = [700, 0, 5000, 130], [0, 0, 4700, 2]
+    heads, kvh, dim, rot, bpp = 16, 2, 128, 64, 2
+    pages = torch.randperm(40, generator=g)[:16].view(4, 4)
+    total = sum(scheduled)
+    want = R.step_tables(computed, scheduled, offsets, pages.tolist(), bpp, total, 8)
+    x = torch.randn(total, (heads + 2 * kvh) * dim, generator=g).to(BF16)
+    kc, vc = (torch.randn(80, 128, kvh, dim, generator=g).to(BF16) for _ in range(2))
+    omega = 1e7 ** (-torch.arange(rot // 2) / (rot // 2))
+    t = K.step_tables(ints(computed), ints(scheduled), pages.int().cuda(), num_tokens=total, max_blocks=8,
+                      offsets=ints(offsets, torch.int64), blocks_per_page=bpp)
+    check_tables(t, want)
+    gk, gv = kc.cuda(), vc.cuda()
+    q, k, v = (y.unflatten(1, (-1, dim)) for y in x.cuda().split([heads * dim, kvh * dim, kvh * dim], 1))
+    q = K.rotary_write(q, k, v, t.positions, t.slot_mapping, gk, gv, omega=omega.cuda())
+    got = K.paged_attention(q, gk, gv, t.block_table, t.query_start_loc, t.seq_lens, max_query_len=max(scheduled),
+                            return_lse=True)
+    # each stage against its 64-bit form, on what the stage before left
+    hq, hk, hv = (y.unflatten(1, (-1, dim)) for y in x.split([heads * dim, kvh * dim, kvh * dim], 1))
+    pos, slots, axis = torch.tensor([want[2]]), torch.tensor(want[3]), torch.zeros(rot // 2).long()
+    assert (q.cpu().double() - R.rotate(hq, pos, omega, axis)).abs().le(R.rotate_bound(hq, omega, BF16)).all()
+    gk, gv = gk.cpu(), gv.cpu()
+    assert (gk.flatten(0, 1)[slots].double() - R.rotate(hk, pos, omega, axis)).abs().le(
+        R.rotate_bound(hk, omega, BF16)).all()
+    assert torch.equal(gv.flatten(0, 1)[slots], hv)
+    c = {"q": q.cpu(), "kc": gk, "vc": gv, "table": torch.tensor(want[5]), "starts": want[0], "lens": want[1]}
+    check_attention(c, got)

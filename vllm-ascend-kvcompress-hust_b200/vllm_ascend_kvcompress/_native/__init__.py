@@ -71,6 +71,18 @@ _SIGNATURES = {
         c_int, [_P, _P, c_int, c_int64, _P, c_int64, _P, _P, _P, c_int, c_int, _P, _P]),
     "kvc_expand_block_ids": (c_int, [_P, c_int64, c_int, _P, _P]),
     "kvc_stage_commit": (c_int, [_P, _P, c_int, c_int, _P, c_int, _P, _P, c_int, _P]),
+    "kvc_step_tables": (
+        c_int, [_P, c_int, _P, c_int, _P, c_int, _P, c_int, c_int64, c_int, c_int, c_int64, c_int, _P, _P, _P, _P,
+                _P, _P, _P, _P]),
+    "kvc_rotary_write": (
+        c_int, [_P, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int64, c_int64, c_int, c_int64, c_int, c_int,
+                c_int, c_int, _P, c_int, c_int64, _P, _P, _P, _P, c_int64, c_int64, _P, c_int64, _P, c_int64,
+                c_int64, _P, _P]),
+    "kvc_paged_attention_workspace_bytes": (c_int64, [c_int, c_int, c_int, c_int]),
+    "kvc_paged_attention": (
+        c_int, [_P, c_int64, c_int64, c_int, c_int64, c_int, c_int, c_int, c_int, _P, c_int64, _P, c_int64, c_int64,
+                _P, c_int64, c_int, _P, _P, c_int, c_float, c_int, c_int, _P, c_int64, c_int64, _P, _P, c_int64, _P,
+                _P]),
     "kvc_calibration_accumulate_noalloc": (
         c_int, [_P, c_int, c_int64, c_int64, c_int, c_int, c_int, _P, _P, _P, _P, _P]),
     "kvc_tp_exchange_flag_words": (c_int, [c_int]),

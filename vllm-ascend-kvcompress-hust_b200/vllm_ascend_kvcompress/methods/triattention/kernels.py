@@ -28,10 +28,15 @@ decode_offsets                 provider.py:687-728 (slot-mapping positions and
                                seq_lens of compressed requests per decode step)
 expand_block_ids               _expand_scheduler_block_ids (provider.py:1273-1287)
 =============================  =====================================================
+
+``step_tables``, ``rotary_write`` and ``paged_attention`` have no counterpart
+there (the reference leaves attention layers to vLLM): they run a serving step
+over the cache that the ones above compress.
 """
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 
 import torch
@@ -444,3 +449,244 @@ def expand_block_ids(ids: torch.Tensor, blocks_per_page: int, out: torch.Tensor 
     N.check(N.lib().kvc_expand_block_ids(_p(ids), ids.numel(), int(blocks_per_page), _p(out), _stream()),
             "kvc_expand_block_ids")
     return out[:n]
+
+
+# ---- the serving step around the compressed cache -------------------------------
+
+
+def _call(device: torch.device, name: str, *args) -> None:
+    """Run a C entry on ``device``'s current stream, whichever device is current."""
+    index = device.index
+    if _raw_stream is None or _cur_device is None or index != _cur_device():
+        with torch.cuda.device(device):
+            N.check(getattr(N.lib(), name)(*args, torch.cuda.current_stream().cuda_stream), name)
+        return
+    status = getattr(N.lib(), name)(*args, _raw_stream(index))
+    if status:
+        N.check(status, name)
+
+
+def _same_device(device: torch.device, tensors) -> None:
+    for t in tensors:
+        if t is not None and t.device != device:
+            if t.device.type != "cuda":
+                raise RuntimeError("the B200 TriAttention kernels require CUDA tensors (no CPU fallback)")
+            raise RuntimeError("all tensors of a call must be on one device")
+
+
+def _error_word(error_flag: torch.Tensor | None) -> int | None:
+    if error_flag is None:
+        return None
+    if error_flag.dtype != torch.int32 or error_flag.numel() < 1:
+        raise RuntimeError("error_flag must be an int32 tensor")
+    return error_flag.data_ptr()
+
+
+def _paged_cache(cache: torch.Tensor, name: str) -> int:
+    """Block stride in elements of a ``[blocks, 128, heads, dim]`` cache."""
+    _, bs, h, d = cache.shape
+    stride = cache.stride()
+    if bs != BLOCK or stride[1:] != (h * d, d, 1):
+        raise RuntimeError(f"{name} must hold {BLOCK}-token blocks with contiguous inner dims")
+    return stride[0]
+
+
+@dataclass(frozen=True)
+class StepTables:
+    """Device tables of one serving step (``step_tables``).
+
+    query_start_loc [R + 1], seq_lens [R] (physical), request_indices [N] and
+    block_table [R, blocks] int32; positions (semantic) and slot_mapping
+    (physical) [N] int64.
+    """
+
+    query_start_loc: torch.Tensor
+    seq_lens: torch.Tensor
+    positions: torch.Tensor
+    slot_mapping: torch.Tensor
+    request_indices: torch.Tensor
+    block_table: torch.Tensor
+
+    @staticmethod
+    def empty(num_requests: int, num_tokens: int, max_blocks: int, device) -> "StepTables":
+        small = torch.empty(2 * num_requests + 1 + num_tokens + num_requests * max_blocks, dtype=torch.int32,
+                            device=device)
+        starts, lens, request, blocks = small.split((num_requests + 1, num_requests, num_tokens,
+                                                     num_requests * max_blocks))
+        positions, slots = torch.empty((2, num_tokens), dtype=torch.int64, device=device).unbind()
+        return StepTables(starts, lens, positions, slots, request, blocks.view(num_requests, max_blocks))
+
+
+_INTS = (torch.int32, torch.int64)
+
+
+def step_tables(computed: torch.Tensor, scheduled: torch.Tensor, page_table: torch.Tensor, *, num_tokens: int,
+                max_blocks: int, offsets: torch.Tensor | None = None, blocks_per_page: int = 1,
+                out: StepTables | None = None, error_flag: torch.Tensor | None = None) -> StepTables:
+    """Block tables, slot map, positions and physical lengths of a step, in one launch.
+
+    ``computed`` and ``scheduled`` [R] (int32 or int64): tokens before the step
+    (semantic) and new ones; ``offsets`` [R] int64: tokens that compression
+    removed; ``page_table`` [R, width] (int32 or int64): scheduler pages of
+    ``128 * blocks_per_page`` tokens.  ``num_tokens`` is the length of the
+    per-token tables (the step's new tokens, or more in a captured step: entries
+    past the last token get slot and request -1) and ``max_blocks`` the width of
+    the block table, whose entries past a request's blocks are -1.  ``out``
+    takes tables of an earlier call or ``StepTables.empty``.
+    """
+    require_cuda(computed, scheduled, page_table, offsets)
+    device = computed.device
+    _same_device(device, (scheduled, page_table, offsets, error_flag))
+    R = computed.numel()
+    if scheduled.numel() != R or page_table.ndim != 2 or page_table.shape[0] != R or (
+            offsets is not None and offsets.numel() != R):
+        raise ValueError("computed, scheduled, offsets and page_table must name the same requests")
+    if not (computed.dtype in _INTS and scheduled.dtype in _INTS and page_table.dtype in _INTS) or not (
+            computed.is_contiguous() and scheduled.is_contiguous() and page_table.stride(1) == 1):
+        raise RuntimeError("computed, scheduled and page_table must be int32 or int64 with unit inner stride")
+    if offsets is not None:
+        _need(offsets, torch.int64, "offsets")
+    if R == 0:
+        raise ValueError("a step has at least one request")
+    if num_tokens < 0 or max_blocks < 0:
+        raise ValueError("num_tokens and max_blocks must not be negative")
+    if out is None:
+        out = StepTables.empty(R, num_tokens, max_blocks, device)
+    else:
+        _same_device(device, (out.query_start_loc, out.seq_lens, out.positions, out.slot_mapping,
+                              out.request_indices, out.block_table))
+        for t, dtype, shape, name in (
+                (out.query_start_loc, torch.int32, (R + 1,), "query_start_loc"),
+                (out.seq_lens, torch.int32, (R,), "seq_lens"),
+                (out.positions, torch.int64, (num_tokens,), "positions"),
+                (out.slot_mapping, torch.int64, (num_tokens,), "slot_mapping"),
+                (out.request_indices, torch.int32, (num_tokens,), "request_indices"),
+                (out.block_table, torch.int32, (R, max_blocks), "block_table")):
+            _need(t, dtype, name)
+            if t.shape != shape:
+                raise ValueError(f"{name} must have shape {shape}")
+    _call(device, "kvc_step_tables", computed.data_ptr(), computed.element_size(), scheduled.data_ptr(),
+          scheduled.element_size(), _p(offsets), R, page_table.data_ptr(), page_table.element_size(),
+          page_table.stride(0), page_table.shape[1], blocks_per_page, num_tokens, max_blocks,
+          out.query_start_loc.data_ptr(), out.seq_lens.data_ptr(), out.positions.data_ptr(),
+          out.slot_mapping.data_ptr(), out.request_indices.data_ptr(), out.block_table.data_ptr(),
+          _error_word(error_flag))
+    return out
+
+
+def rotary_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+                 slot_mapping: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, *, omega: torch.Tensor,
+                 axis_of_frequency: torch.Tensor | None = None, q_out: torch.Tensor | None = None,
+                 error_flag: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotate ``q`` and ``k`` at their positions; keys and values go to their cache slots.
+
+    ``q`` [N, heads, dim], ``k`` and ``v`` [N, kv_heads, dim] (bf16 or fp16,
+    views of a fused projection included); ``positions`` [N] or [axes, N] int64
+    (semantic); ``omega`` [rotary_dim / 2] fp32 with ``axis_of_frequency`` int32
+    naming each frequency's axis when there are several; ``slot_mapping`` [N]
+    int64 (physical; negative: nothing is written); caches
+    ``[blocks, 128, kv_heads, dim]`` with any block stride.  "Half" style pairs,
+    as the calibration statistics assume.  Returns the rotated queries
+    (``q_out``, which may be ``q``; a new tensor by default).
+    """
+    require_cuda(q, k, v, positions, slot_mapping, k_cache, v_cache, omega, axis_of_frequency, q_out)
+    device, dtype = q.device, q.dtype
+    _same_device(device, (k, v, positions, slot_mapping, k_cache, v_cache, omega, axis_of_frequency, q_out,
+                          error_flag))
+    code = _dtype_code(dtype)
+    if q.ndim != 3 or k.ndim != 3 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+        raise ValueError("q must be [tokens, heads, dim], k and v [tokens, kv_heads, dim]")
+    n, heads, dim = q.shape
+    kvh = k.shape[1]
+    if k_cache.ndim != 4 or k_cache.shape != v_cache.shape or k_cache.shape[2:] != (kvh, dim):
+        raise ValueError("caches must be [blocks, 128, kv_heads, dim] of k's heads")
+    if k.dtype != dtype or v.dtype != dtype or k_cache.dtype != dtype or v_cache.dtype != dtype:
+        raise RuntimeError("q, k, v and the caches must have one dtype")
+    if q_out is None:
+        q_out = torch.empty((n, heads, dim), dtype=dtype, device=device)
+    elif q_out.dtype != dtype or q_out.shape != q.shape:
+        raise RuntimeError("q_out must have q's dtype and shape")
+    qs, ks, vs, os = q.stride(), k.stride(), v.stride(), q_out.stride()
+    if qs[2] != 1 or ks[2] != 1 or vs[2] != 1 or os[2] != 1:
+        raise RuntimeError("q, k, v and q_out must have a contiguous last dim")
+    axes = positions.shape[0] if positions.ndim == 2 else 1
+    if positions.dtype != torch.int64 or positions.ndim not in (1, 2) or positions.shape[-1] != n or (
+            n > 1 and positions.stride(-1) != 1):
+        raise RuntimeError("positions must be int64 [tokens] or [axes, tokens] with unit inner stride")
+    _need(slot_mapping, torch.int64, "slot_mapping")
+    if slot_mapping.numel() != n:
+        raise ValueError("slot_mapping must have one slot per token")
+    _need(omega, torch.float32, "omega")
+    if axis_of_frequency is not None:
+        _need(axis_of_frequency, torch.int32, "axis_of_frequency")
+        if axis_of_frequency.numel() != omega.numel():
+            raise ValueError("axis_of_frequency must name one axis per frequency")
+    elif axes > 1:
+        raise ValueError("several axes need axis_of_frequency")
+    _call(device, "kvc_rotary_write", q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0],
+          vs[1], code, n, heads, kvh, dim, 2 * omega.numel(), positions.data_ptr(), axes,
+          positions.stride(0) if axes > 1 else 0, omega.data_ptr(), _p(axis_of_frequency), slot_mapping.data_ptr(),
+          q_out.data_ptr(), os[0], os[1], k_cache.data_ptr(), _paged_cache(k_cache, "k_cache"), v_cache.data_ptr(),
+          _paged_cache(v_cache, "v_cache"), k_cache.shape[0], _error_word(error_flag))
+    return q_out
+
+
+def paged_attention_workspace_bytes(max_query_len: int, heads: int, kv_heads: int, head_dim: int) -> int:
+    return int(N.lib().kvc_paged_attention_workspace_bytes(max_query_len, heads, kv_heads, head_dim))
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                    query_start_loc: torch.Tensor, seq_lens: torch.Tensor, *, max_query_len: int,
+                    scale: float | None = None, window: int = 0, sinks: int = 0, out: torch.Tensor | None = None,
+                    return_lse: bool = False, workspace: torch.Tensor | None = None,
+                    error_flag: torch.Tensor | None = None):
+    """Attention of each request's newest tokens over its paged (possibly compressed) cache.
+
+    ``q`` [N, heads, dim]; request r owns rows ``query_start_loc[r]`` to
+    ``query_start_loc[r + 1]`` and its cache holds ``seq_lens[r]`` physical
+    tokens, the new ones last, in the blocks ``block_table[r]`` (all int32, as
+    ``step_tables`` makes them).  A token at physical position p sees keys up
+    to p; with ``window`` > 0 only the last ``window`` of them and the first
+    ``sinks`` tokens of the cache.  ``scale`` defaults to ``dim ** -0.5``.
+    ``max_query_len`` is the most new tokens of a request.  Returns ``out``
+    [N, heads, dim], or ``(out, lse)`` with the fp32 logarithm of each row's sum
+    of exponentials.  ``workspace`` (``paged_attention_workspace_bytes``) is
+    allocated per call unless given; one given must not serve two calls that
+    run at the same time.
+    """
+    require_cuda(q, k_cache, v_cache, block_table, query_start_loc, seq_lens, out, workspace)
+    device, dtype = q.device, q.dtype
+    _same_device(device, (k_cache, v_cache, block_table, query_start_loc, seq_lens, out, workspace, error_flag))
+    code = _dtype_code(dtype)
+    if q.ndim != 3 or k_cache.ndim != 4 or k_cache.shape != v_cache.shape or k_cache.shape[3] != q.shape[2]:
+        raise ValueError("q must be [tokens, heads, dim] and the caches [blocks, 128, kv_heads, dim]")
+    if k_cache.dtype != dtype or v_cache.dtype != dtype:
+        raise RuntimeError("q and the caches must have one dtype")
+    n, heads, dim = q.shape
+    kvh, R = k_cache.shape[2], seq_lens.numel()
+    _need(query_start_loc, torch.int32, "query_start_loc")
+    _need(seq_lens, torch.int32, "seq_lens")
+    if query_start_loc.numel() != R + 1 or block_table.ndim != 2 or block_table.shape[0] != R:
+        raise ValueError("query_start_loc, seq_lens and block_table must name the same requests")
+    if block_table.dtype != torch.int32 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise RuntimeError("block_table must be int32 with unit inner stride")
+    if out is None:
+        out = torch.empty((n, heads, dim), dtype=dtype, device=device)
+    elif out.dtype != dtype or out.shape != q.shape:
+        raise RuntimeError("out must have q's dtype and shape")
+    qs, os = q.stride(), out.stride()
+    if qs[2] != 1 or os[2] != 1:
+        raise RuntimeError("q and out must have a contiguous last dim")
+    lse = torch.empty((n, heads), dtype=torch.float32, device=device) if return_lse else None
+    if workspace is None:
+        size = N.lib().kvc_paged_attention_workspace_bytes(max_query_len, heads, kvh, dim)
+        workspace = torch.empty(size, dtype=torch.uint8, device=device)
+    elif not workspace.is_contiguous():
+        raise RuntimeError("workspace must be contiguous")
+    _call(device, "kvc_paged_attention", q.data_ptr(), qs[0], qs[1], code, n, max_query_len, heads, kvh, dim,
+          k_cache.data_ptr(), _paged_cache(k_cache, "k_cache"), v_cache.data_ptr(), _paged_cache(v_cache, "v_cache"),
+          k_cache.shape[0], block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+          query_start_loc.data_ptr(), seq_lens.data_ptr(), R, 1.0 / math.sqrt(dim) if scale is None else scale,
+          window, sinks, out.data_ptr(), os[0], os[1], _p(lse), workspace.data_ptr(),
+          workspace.numel() * workspace.element_size(), _error_word(error_flag))
+    return (out, lse) if return_lse else out
