@@ -36,7 +36,7 @@ constexpr int kSpan = 64;  // elements of a 128-byte swizzle span
 
 template <int D>
 struct Geom {
-  static constexpr int KB = D <= 128 ? 128 : 64;   // keys per unit
+  static constexpr int KB = D <= 128 ? 128 : 64;   // keys per unit (rows_keys)
   static constexpr int kTile = KB * D * 2;         // bytes of a K (or V) block
   static constexpr int kStage = 2 * kTile;
   static constexpr int kMerge = kConsumers * kRows * D * 4;
@@ -471,10 +471,34 @@ int encode_cache_map(CUtensorMap* map, const void* cache, bool fp16, int D, int 
   return rc == CUDA_SUCCESS ? KVC_OK : KVC_ECUDA;
 }
 
+// [token][head][dim], boxes of 64 dims x the heads of a KV head x a tile half's tokens
+int encode_query_map(CUtensorMap* map, const AttendArgs& a, bool fp16) {
+  PFN_cuTensorMapEncodeTiled_v12000 fn = encode_fn();
+  if (!fn) return KVC_ECUDA;
+  const cuuint64_t dims[3] = {(cuuint64_t)a.D, (cuuint64_t)a.Hq, (cuuint64_t)a.num_tokens};
+  const cuuint64_t strides[2] = {(cuuint64_t)a.q_head * 2, (cuuint64_t)a.q_tok * 2};
+  const cuuint32_t box[3] = {(cuuint32_t)kSpan, (cuuint32_t)a.G, (cuuint32_t)a.sub};
+  const cuuint32_t one[3] = {1, 1, 1};
+  const CUresult rc =
+      fn(map, fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<uint16_t*>(a.q),
+         dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return rc == CUDA_SUCCESS ? KVC_OK : KVC_ECUDA;
+}
+
+constexpr int rows_keys(int D) { return D <= 128 ? 128 : 64; }
+
 }  // namespace
 }  // namespace kvc
 
 using namespace kvc;
+
+// Rows of a tile.  Up to 16 rows in the longest request: the 16-row kernel,
+// which streams a decode step's caches at 0.9 of the copy rate.  More: the
+// tcgen05 kernel, whose products are 128 rows wide whatever the rows in use.
+static int tile_rows(int max_query_len, int group, int head_dim) {
+  return (int64_t)max_query_len * group <= kRows ? kRows : attend_umma_rows(head_dim);
+}
 
 // Workspace: parts' outputs, their (m, l), and one record per CTA.
 static int64_t workspace_bytes(int ctas, int rows, int D) {
@@ -485,7 +509,7 @@ extern "C" int64_t kvc_paged_attention_workspace_bytes(int max_query_len, int he
   if (max_query_len < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads / kv_heads > kRows ||
       (head_dim != 64 && head_dim != 128 && head_dim != 256))
     return 0;
-  return workspace_bytes(sm_count(), kRows, head_dim);
+  return workspace_bytes(sm_count(), tile_rows(max_query_len, heads / kv_heads, head_dim), head_dim);
 }
 
 extern "C" int kvc_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype,
@@ -512,14 +536,15 @@ extern "C" int kvc_paged_attention(const void* q, int64_t q_token_stride, int64_
   KVC_CHECK_ARG(k_block_stride >= page && v_block_stride >= page, KVC_EINVAL);
   const int64_t strides[] = {q_token_stride, q_head_stride, out_token_stride, out_head_stride, k_block_stride,
                              v_block_stride};
-  for (int64_t s : strides) KVC_CHECK_ARG(s >= 0 && s % 8 == 0, KVC_EALIGN);
+  for (int64_t s : strides) KVC_CHECK_ARG(s > 0 && s % 8 == 0, KVC_EALIGN);
   const void* ptrs[] = {q, k_cache, v_cache, out, workspace};
   for (const void* p : ptrs) KVC_CHECK_ARG(aligned(p, 16), KVC_EALIGN);
   KVC_CHECK_ARG(aligned(lse, 4) && aligned(block_table, 4), KVC_EALIGN);
   AttendArgs a{};
   const bool fp16 = dtype == KVC_FP16;
   a.ctas = sm_count();
-  a.rows = kRows;
+  a.rows = tile_rows(max_query_len, heads / kv_heads, head_dim);
+  const bool wide = a.rows != kRows;
   KVC_CHECK_ARG(workspace_size >= workspace_bytes(a.ctas, a.rows, head_dim), KVC_EINVAL);
   a.q = (const uint16_t*)q;
   a.out = (uint16_t*)out;
@@ -536,15 +561,17 @@ extern "C" int kvc_paged_attention(const void* q, int64_t q_token_stride, int64_
   a.num_tokens = num_tokens;
   a.R = num_requests, a.Hq = heads, a.Hkv = kv_heads, a.G = heads / kv_heads, a.D = head_dim;
   a.window = window, a.sinks = window > 0 ? sinks : 0;
-  a.tok = kRows / a.G;
+  a.sub = 128 / a.G;
+  a.tok = wide ? a.rows / 128 * a.sub : kRows / a.G;
   a.min_units = 1;
   a.scale = scale;
   a.scale_log2 = scale * 1.44269504088896340736f;
-  const int keys = head_dim <= 128 ? 128 : 64;
+  const int keys = wide ? attend_umma_slot_keys(head_dim) : rows_keys(head_dim);
   int rc = encode_cache_map(&a.kmap, k_cache, fp16, head_dim, kv_heads, k_block_stride, num_blocks, keys);
   if (rc == KVC_OK)
     rc = encode_cache_map(&a.vmap, v_cache, fp16, head_dim, kv_heads, v_block_stride, num_blocks, keys);
-  if (rc == KVC_OK) rc = rows_launch(a, fp16, (cudaStream_t)stream);
+  if (rc == KVC_OK && wide) rc = encode_query_map(&a.qmap, a, fp16);
+  if (rc == KVC_OK) rc = wide ? attend_umma_launch(a, fp16, (cudaStream_t)stream) : rows_launch(a, fp16, (cudaStream_t)stream);
   if (rc == KVC_OK) rc = combine_launch(a, fp16, (cudaStream_t)stream);
   return rc;
 }

@@ -49,6 +49,7 @@ struct AttendArgs {
   int R, Hq, Hkv, G, D;
   int window, sinks;
   int tok;   // tokens per tile
+  int sub;   // tokens per 128-row half of a tile (tcgen05 kernel)
   int rows;  // rows of a partial
   int ctas;  // CTAs that share the line of units
   int min_units;
@@ -247,5 +248,10 @@ __device__ __forceinline__ float exp2_approx(float x) {
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn();  // kvc_score_tc.cu
+
+// kvc_attend_umma.cu: tiles of up to 256 rows
+int attend_umma_rows(int D);       // rows of a tile
+int attend_umma_slot_keys(int D);  // keys of a K/V box
+int attend_umma_launch(const AttendArgs& a, bool fp16, cudaStream_t st);
 
 }  // namespace kvc
