@@ -58,34 +58,25 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int32_t
   }
 }
 
-__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-
-// A short wait for loops that have to stay in the instruction cache, bounded by
-// a count: a try that fails suspends the thread for some 4 us (measured: 7,765
-// cycles), so kWaitTries of them are about kWaitNs.
-constexpr uint32_t kWaitTries = 1u << 19;
-
+// The same wait with its loop kept small, for loops that have to stay in the
+// instruction cache: the timer is looked at after every 64 tries.
 __device__ __forceinline__ bool mbar_wait_short(uint32_t bar, uint32_t parity, int32_t* flag) {
+  uint64_t start = 0;
 #pragma unroll 1
-  for (uint32_t i = 0; i < kWaitTries; ++i)
-    if (mbar_try(bar, parity)) return true;
-  raise_flag(flag, KVC_DEV_TIMEOUT);
-  return false;
-}
-
-// The lanes of a warp wait together.
-__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, int32_t* flag) {
-#pragma unroll 1
-  for (uint32_t i = 0; i < kWaitTries; ++i)
-    if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
+  for (;;) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, 64;\n"
+        "W:\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra D;\n\t"
+        "sub.u32 n, n, 1;\n\tsetp.ne.u32 q, n, 0;\n\t@q bra W;\n"
+        "D:\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (__builtin_expect(ok, 1)) return true;
+    if (start == 0) start = global_ns();
+    else if (global_ns() - start > kWaitNs) break;
+  }
   raise_flag(flag, KVC_DEV_TIMEOUT);
   return false;
 }

@@ -49,13 +49,12 @@ static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * kLaunchRegs, "registers");
 constexpr int KB = 128;                 // keys per unit
 constexpr int kSpan = 64;               // elements of a 128-byte swizzle span
 constexpr int kMeta = 16;
-constexpr float kSlack = 8.f;           // log2 of the largest weight
+constexpr float kSlack = 8.f;           // a maximum is raised for scores this far above it (log2 of their weight)
+constexpr float kMost = 32768.f;        // and for 64 weights with a larger sum
 
 template <int D>
 struct Geom {
   static constexpr int NT = D <= 128 ? 2 : 1;      // 128-row halves
-  // P beside S in TMEM (the next S may then be computed once this one is read), or over it
-  static constexpr bool kBeside = D != 128;
   static constexpr int SK = D <= 128 ? 128 : 64;   // keys of a ring slot
   static constexpr int HV = KB / SK;               // slots of a K (or V) block
   static constexpr int kSlot = SK * D * 2;
@@ -63,25 +62,25 @@ struct Geom {
   static constexpr int kQ = 128 * D * 2;           // queries of a half
   static constexpr int kFit = (225 * 1024 - NT * kQ) / kSlot;
   static constexpr int S = kFit > 10 ? 10 : kFit;
-  static constexpr int SC = NT == 2 ? KB : KB / 2;  // S columns of a softmax thread
-  static constexpr int OC = NT == 2 ? D : D / 2;    // O columns of a softmax thread
-  static constexpr int kBars = 2 * S + 15;
+  static constexpr int OC = NT == 2 ? D : D / 2;   // O columns of a softmax thread
+  // barriers, 8 bytes each: places in their array
+  enum Bar : int { kFull = 0, kEmpty = S, kQFull = 2 * S, kQEmpty, kSFull, kPFull = kSFull + 4, kODone = kPFull + 4,
+                   kSRead = kODone + 4, kOFree, kDone = kOFree + 2, kBars };
   static constexpr int kTail = kBars * 8 + kMeta * 4 + 16 + (NT == 1 ? 2048 : 0);
   static constexpr int kSmem = NT * kQ + S * kSlot + kTail;
   static_assert(S >= 5 && kSmem <= 227 * 1024 && kSmem > 116 * 1024, "one CTA per SM: it holds every TMEM column");
   static_assert(S * kSlot >= (kMaxAttendRequests + 41) * 4, "the prefix sums lie in the ring");
-  // TMEM columns: S of the halves, P (of the halves, or of even and odd units), O
-  static __device__ __forceinline__ uint32_t s_col(int half) { return 128 * half; }
-  static __device__ __forceinline__ uint32_t p_col(int half, uint32_t g) {
-    return NT == 1 ? 128 + 64 * (g & 1) : kBeside ? 256 + 2 * D + 64 * half : 128 * half;
+  // TMEM columns.  Two halves: S of a half's 64-key parts, P over the S it came from.  One: S of 128 keys, P
+  // of even and odd units.  O from 256 on.
+  static __device__ __forceinline__ uint32_t s_col(int half, int part) { return 128 * half + 64 * part; }
+  static __device__ __forceinline__ uint32_t p_col(int half, int part, uint32_t g) {
+    return NT == 2 ? 128 * half + 64 * part : 128 + 64 * (g & 1) + 32 * part;
   }
   static __device__ __forceinline__ uint32_t o_col(int half) { return 256 + D * half; }
-  static_assert(NT == 1 || 256 + 2 * D + (kBeside ? 128 : 0) <= 512, "TMEM columns");
-  // Place of unit g's K and V among the 2 n blocks of the CTA's n units, as the MMA warp takes them:
-  // K(g), V(g), .. with P over S, else K(g + 1) before V(g)
-  static __device__ __forceinline__ uint32_t k_at(uint32_t g) { return !kBeside ? 2 * g : g == 0 ? 0 : 2 * g - 1; }
+  // place of unit g's K and V among the 2 n blocks of the CTA's n units, as the MMA warps take them
+  static __device__ __forceinline__ uint32_t k_at(uint32_t g) { return NT == 2 ? 2 * g : g == 0 ? 0 : 2 * g - 1; }
   static __device__ __forceinline__ uint32_t v_at(uint32_t g, uint32_t n) {
-    return !kBeside ? 2 * g + 1 : g + 1 == n ? 2 * n - 1 : 2 * g + 2;
+    return NT == 2 ? 2 * g + 1 : g + 1 == n ? 2 * n - 1 : 2 * g + 2;
   }
 };
 
@@ -149,14 +148,15 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
   extern __shared__ __align__(1024) uint8_t base[];
   const uint32_t q0 = smem_u32(base), ring0 = q0 + NT * G_::kQ;
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + NT * G_::kQ + S * G_::kSlot);
-  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * S;
-  const uint32_t qfull = empty0 + 8 * S, qempty = qfull + 8;
-  const uint32_t sfull = qempty + 8;   // [half] S is complete
-  const uint32_t sread = sfull + 16;   // [half] S has been read (P beside S)
-  const uint32_t pfull = sread + 16;   // [half][2] P of the first and of the last 64 keys is in place
-  const uint32_t odone = pfull + 32;   // [half], or [unit & 1] with one half: P V is complete
-  const uint32_t ofree = odone + 16;   // [half] the tile's output has been read
-  const uint32_t done = ofree + 16;
+  const uint32_t full0 = smem_u32(bars);
+  const uint32_t empty0 = full0 + 8 * G_::kEmpty;
+  const uint32_t qfull = full0 + 8 * G_::kQFull, qempty = full0 + 8 * G_::kQEmpty;
+  const uint32_t sfull = full0 + 8 * G_::kSFull;  // [half][part] S is complete (one half: [0][0])
+  const uint32_t pfull = full0 + 8 * G_::kPFull;  // [half][part] P is in its place
+  const uint32_t odone = full0 + 8 * G_::kODone;  // [half][part], or [unit & 1] with one half: P V is complete
+  const uint32_t sread = full0 + 8 * G_::kSRead;  // S has been read (one half)
+  const uint32_t ofree = full0 + 8 * G_::kOFree;  // [half] the tile's output has been read
+  const uint32_t done = full0 + 8 * G_::kDone;    // every product is complete
   volatile uint32_t* meta = reinterpret_cast<uint32_t*>(bars + G_::kBars);  // per unit, from the producer
   uint32_t* tmem_slot = const_cast<uint32_t*>(meta + kMeta);
   float* xch = reinterpret_cast<float*>(tmem_slot + 4);  // [2][2][128] (NT == 1)
@@ -176,14 +176,13 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
     }
     mbar_init(qfull, 1);
     mbar_init(qempty, NT);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       mbar_init(sfull + 8 * i, 1);
-      mbar_init(sread + 8 * i, NT == 2 ? 4 : 8);  // softmax warps arrive once each
-      mbar_init(pfull + 16 * i, 4);               // with one half, each warpgroup has 64 of the keys
-      mbar_init(pfull + 16 * i + 8, 4);
+      mbar_init(pfull + 8 * i, 4);  // softmax warps arrive once each
       mbar_init(odone + 8 * i, 1);
-      mbar_init(ofree + 8 * i, NT == 2 ? 4 : 8);
     }
+    mbar_init(sread, 8);
+    for (int i = 0; i < 2; ++i) mbar_init(ofree + 8 * i, NT == 2 ? 4 : 8);
     mbar_init(done, 2);
     mbar_init_fence();
   }
@@ -224,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
           }
           return true;
         };
-        int prev_blk = -1, prev_h = 0;  // the unit whose V is still to come (P beside S)
+        int prev_blk = -1, prev_h = 0;  // (one half) the unit whose V is still to come
         while (ok && c.left > 0) {
           const AttendTile t = attend_tile<KB>(a, c.r, c.i);
           const int n = (int)min64(t.units - c.u, c.left);
@@ -241,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
             meta[g % kMeta] = (blk < 0 ? kSkip : 0) | (u == 0 ? kFirst : 0) | (u + 1 == n ? kLast : 0) |
                               (halves == 2 ? kTwo : 0);
             ok = fill(&a.kmap, c.h, blk);
-            if constexpr (!G_::kBeside) {
+            if constexpr (NT == 2) {
               ok = ok && fill(&a.vmap, c.h, blk);
             } else {
               if (g > 0) ok = ok && fill(&a.vmap, prev_h, prev_blk);
@@ -252,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
           c.left -= n;
           if (c.left > 0) attend_advance(a, c);
         }
-        if constexpr (G_::kBeside) {
+        if constexpr (NT == 1) {
           if (ok && g > 0) fill(&a.vmap, prev_h, prev_blk);
         }
         // every copy has landed before the CTA may end
@@ -264,131 +263,175 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
       }
       __syncwarp();
     } else if (warp <= kMma + 1) {
-      // ---------------- MMA issuers: a warp each for the two halves, or for S and for O with one half ----------------
-      // The warp walks along, one lane issues.  An issued product holds the lane until the tensor pipe takes
-      // it, and a wait that is met takes some 100 cycles: with one warp for everything the pipe stood still
-      // through the waits of one half where the other's products were ready.
-      constexpr uint32_t id_s = idesc(FP16, SK, false), id_o = idesc(FP16, D, true);
-      const int role = warp - kMma;
-      const int half = NT == 2 ? role : 0;
-      auto wait = [&](uint32_t bar, uint32_t parity) { return mbar_wait_warp(bar, parity, a.error_flag); };
-      uint32_t pieces = 0;                      // whose queries have been waited for
-      uint32_t n_qk = 0, n_pv = 0, n_o = 0;     // units and pieces of this half
-      // S = Q K of unit g, whose flags go to f
-      auto qk = [&](uint32_t g, uint32_t& f) {
-        const uint32_t seq = HV * G_::k_at(g);
-        if (!wait(full0 + 8 * (seq % S), (seq / S) & 1)) return false;
-        f = meta[g % kMeta];
-        if ((f & kFirst) && !wait(qfull, pieces++ & 1)) return false;
-        const bool idle = half == 1 && !(f & kTwo);  // a tile without a second half: its blocks pass by
-        if (!idle && G_::kBeside && n_qk > 0 && !wait(sread + 8 * half, (n_qk - 1) & 1)) return false;
-        if (!idle) ++n_qk;
-#pragma unroll 1
-        for (int hv = 0; hv < HV; ++hv) {
-          const uint32_t s = (seq + hv) % S;
-          if (hv > 0 && !wait(full0 + 8 * s, ((seq + hv) / S) & 1)) return false;
-          tc_fence_after();
-          if (elect_one()) {
-            if (!idle && !(f & kSkip)) {
-              const uint64_t qd = sw128_desc(q0 + half * G_::kQ), kd = sw128_desc(ring0 + s * G_::kSlot);
+      // ---------------- MMA issuers: a lane each for the two halves, or for S and for O with one half ----------------
+      // An issued product holds the lane until the tensor pipe takes it, and with one lane for everything the
+      // pipe stood still through the waits of one half where the other's products were ready.  A wait that is
+      // met takes the lane through some 20 dependent instructions, so slots and phases are carried along
+      // instead of divided out.
+      if (elect_one()) {
+        constexpr uint32_t id_s = idesc(FP16, 64, false), id_o = idesc(FP16, D, true);
+        const int role = warp - kMma;
+        const int half = NT == 2 ? role : 0;
+        bool ok = true;
+        auto wait = [&](uint32_t bar, uint32_t parity) {
+          if (ok) ok = mbar_wait_short(bar, parity, a.error_flag);
+        };
+        auto advance = [&](uint32_t& s, uint32_t& parity, uint32_t by) {  // a slot and its phase
+          s += by;
+          if (s >= S) {
+            s -= S;
+            parity ^= 1;
+          }
+        };
+        const uint64_t qd = sw128_desc(q0 + half * G_::kQ), ring_k = sw128_desc(ring0),
+                       ring_v = sw128_mn_desc(ring0, G_::kBox);  // start addresses count 16 bytes
+        auto qk = [&](uint32_t d, uint64_t kd) {  // S of 64 keys
 #pragma unroll
-              for (int k = 0; k < D / 16; ++k)  // start addresses count 16 bytes
-                mma_ss(tmem + G_::s_col(half) + hv * SK, qd + (k >> 2) * (128 * 128 / 16) + (k & 3) * 2,
-                       kd + (k >> 2) * (G_::kBox / 16) + (k & 3) * 2, id_s, k > 0 ? 1u : 0u);
-            }
-            tc_commit(empty0 + 8 * s);
-            if (hv == HV - 1) {
-              if (!idle) tc_commit(sfull + 8 * half);
-              if (f & kLast) tc_commit(qempty);
-            }
-          }
-        }
-        return true;
-      };
-      // O (+)= P V of unit g; P comes in two parts of 64 keys
-      auto pv = [&](uint32_t g, uint32_t f, bool& acc) {
-        const uint32_t seq = HV * G_::v_at(g, units), par = n_pv & 1;
-        if constexpr (NT == 1) {
-          // Both parts first: either warpgroup may still be rescaling its columns of O.  What was in V's slots
-          // before has arrived for certain only then, so that the barrier's phase means this V; and the
-          // unit's flags have.
-          if (!(wait(pfull, par) && wait(pfull + 8, par))) return false;
-          f = meta[g % kMeta];
-        }
-        const bool idle = half == 1 && !(f & kTwo);
-        if (!idle && (f & kFirst) && !wait(ofree + 8 * half, (n_o++ & 1) ^ 1)) return false;
-        if (f & kFirst) acc = false;
-        if (!idle) ++n_pv;
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t s = (seq + (HV == 2 ? h : 0)) % S;
-          if constexpr (NT == 1) {
-            if (!wait(full0 + 8 * s, ((seq + h) / S) & 1)) return false;
-          } else {
-            if (h == 0 && !wait(full0 + 8 * s, (seq / S) & 1)) return false;
-            if (!idle && !wait(pfull + 16 * half + 8 * h, par)) return false;
-          }
-          tc_fence_after();
-          if (elect_one()) {
-            if (!idle && !(f & kSkip)) {
-              const uint64_t vd =
-                  sw128_mn_desc(ring0 + s * G_::kSlot, G_::kBox) + (HV == 1 ? h * (4 * 2048 / 16) : 0);
+          for (int k = 0; k < D / 16; ++k)
+            mma_ss(d, qd + (k >> 2) * (128 * 128 / 16) + (k & 3) * 2, kd + (k >> 2) * (G_::kBox / 16) + (k & 3) * 2,
+                   id_s, k > 0 ? 1u : 0u);
+        };
+        auto pv = [&](uint32_t p, uint64_t vd, bool acc) {  // O (+)= P V of 64 keys
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                mma_ts(tmem + G_::o_col(half), tmem + G_::p_col(half, g) + h * 32 + 8 * k, vd + k * (2048 / 16), id_o,
-                       acc || h + k > 0 ? 1u : 0u);
+          for (int k = 0; k < 4; ++k)
+            mma_ts(tmem + G_::o_col(half), p + 8 * k, vd + k * (2048 / 16), id_o, acc || k > 0 ? 1u : 0u);
+        };
+        uint32_t pieces = 0, n_o = 0;  // whose queries, whose place for the output have been waited for
+        bool acc = false;
+        if constexpr (NT == 2) {
+          // Parts of 64 keys: S of the next part runs under this one's softmax, in the buffer that the part
+          // before this one has left.  Products of different shapes have no order among each other, so that
+          // part's P V is waited for.
+          const uint32_t s_bar = sfull + 16 * half, p_bar = pfull + 16 * half, o_bar = odone + 16 * half;
+          uint32_t ks = 0, kp = 0, vs = 1, vp = 0;
+          uint32_t f = 0, n = 0;  // flags of the unit; units of this half
+          auto first_part = [&](uint32_t g, uint32_t n) {  // S of unit g's first 64 keys; the unit's flags
+            wait(full0 + 8 * ks, kp);
+            const uint32_t nf = meta[g % kMeta];
+            if (nf & kFirst) wait(qfull, pieces++ & 1);
+            if (half == 0 || (nf & kTwo)) {
+              if (n > 0) wait(o_bar, (n - 1) & 1);
+              tc_fence_after();
+              if (ok && !(nf & kSkip)) qk(tmem + G_::s_col(half, 0), ring_k + ks * (G_::kSlot / 16));
+              tc_commit(s_bar);
             }
-            if (HV == 2 || h == 1) tc_commit(empty0 + 8 * s);
-            if (h == 1 && !idle) tc_commit(odone + 8 * (NT == 1 ? (g & 1) : half));
+            return nf;
+          };
+          if (units > 0) f = first_part(0, 0);
+          for (uint32_t g = 0; ok && g < units; ++g) {
+            const bool live = half == 0 || (f & kTwo);  // a tile without a second half: its blocks pass by
+            const bool more = g + 1 < units;
+            uint32_t nf = 0;
+            if (live) {
+              if (n > 0) wait(o_bar + 8, (n - 1) & 1);
+              tc_fence_after();
+              if (ok && !(f & kSkip)) qk(tmem + G_::s_col(half, 1), ring_k + ks * (G_::kSlot / 16) + 64 * 128 / 16);
+              tc_commit(s_bar + 8);
+            }
+            tc_commit(empty0 + 8 * ks);
+            if (f & kLast) tc_commit(qempty);
+            advance(ks, kp, 2);
+            if (live && (f & kFirst)) {
+              wait(ofree + 8 * half, (n_o++ & 1) ^ 1);
+              acc = false;
+            }
+            wait(full0 + 8 * vs, vp);
+            if (live) {
+              wait(p_bar, n & 1);
+              tc_fence_after();
+              if (ok && !(f & kSkip)) pv(tmem + G_::p_col(half, 0, g), ring_v + vs * (G_::kSlot / 16), acc);
+              tc_commit(o_bar);
+              acc = acc || !(f & kSkip);
+            }
+            // at a tile's end the next queries are still on their way: P V first
+            if (more && !(f & kLast)) nf = first_part(g + 1, n + live);
+            if (live) {
+              wait(p_bar + 8, n & 1);
+              tc_fence_after();
+              if (ok && !(f & kSkip)) pv(tmem + G_::p_col(half, 1, g), ring_v + vs * (G_::kSlot / 16) + 64 * 128 / 16, acc);
+              tc_commit(o_bar + 8);
+            }
+            tc_commit(empty0 + 8 * vs);
+            advance(vs, vp, 2);
+            if (more && (f & kLast)) nf = first_part(g + 1, n + live);
+            n += live;
+            f = nf;
+          }
+        } else if (role == 0) {
+          uint32_t ks = 0, kp = 0;
+          for (uint32_t g = 0; ok && g < units; ++g) {
+            wait(full0 + 8 * ks, kp);
+            const uint32_t f = meta[g % kMeta];
+            if (f & kFirst) wait(qfull, pieces++ & 1);
+            if (g > 0) wait(sread, (g - 1) & 1);
+#pragma unroll 1
+            for (int hv = 0; hv < 2; ++hv) {
+              if (hv > 0) wait(full0 + 8 * ks, kp);
+              tc_fence_after();
+              if (ok && !(f & kSkip)) qk(tmem + G_::s_col(0, hv), ring_k + ks * (G_::kSlot / 16));
+              tc_commit(empty0 + 8 * ks);
+              advance(ks, kp, 1);
+            }
+            tc_commit(sfull);
+            if (f & kLast) tc_commit(qempty);
+            if (g > 0) advance(ks, kp, 2);  // V(g - 1) lies between K(g) and K(g + 1)
+          }
+        } else {
+          uint32_t vs = 0, vp = 0;
+          advance(vs, vp, units > 1 ? 4 : 2);  // K(0), K(1), V(0), K(2), V(1), ..
+          for (uint32_t g = 0; ok && g < units; ++g) {
+            // P first: either warpgroup may still be rescaling its columns of O.  What was in V's slots before
+            // has arrived for certain only then, so that the barrier's phase means this V; and the unit's
+            // flags have.
+            wait(pfull, g & 1);
+            wait(pfull + 8, g & 1);
+            const uint32_t f = meta[g % kMeta];
+            if (f & kFirst) {
+              wait(ofree, (n_o++ & 1) ^ 1);
+              acc = false;
+            }
+#pragma unroll 1
+            for (int hv = 0; hv < 2; ++hv) {
+              wait(full0 + 8 * vs, vp);
+              tc_fence_after();
+              if (ok && !(f & kSkip)) pv(tmem + G_::p_col(0, hv, g), ring_v + vs * (G_::kSlot / 16), acc || hv > 0);
+              tc_commit(empty0 + 8 * vs);
+              advance(vs, vp, 1);
+            }
+            tc_commit(odone + 8 * (g & 1));
+            acc = acc || !(f & kSkip);
+            if (g + 2 < units) advance(vs, vp, 2);  // K(g + 2) lies between V(g) and V(g + 1)
           }
         }
-        acc = acc || !(f & kSkip);
-        return true;
-      };
-      uint32_t f = 0, nf = 0;
-      bool acc = false, ok = true;
-      if constexpr (NT == 2) {
-        ok = units == 0 || qk(0, f);
-        for (uint32_t g = 0; ok && g < units; ++g) {
-          // P beside S: the next S comes first and runs under this unit's softmax, but for a tile's end,
-          // where the next queries are still on their way.  P over S: the next S has to come second.  (Both
-          // are this thread's, of one shape, and execute in the order of issue.)
-          const bool more = g + 1 < units, early = G_::kBeside && more && !(f & kLast);
-          if (early) ok = qk(g + 1, nf);
-          ok = ok && pv(g, f, acc);
-          if (more && !early) ok = ok && qk(g + 1, nf);
-          f = nf;
-        }
-      } else if (role == 0) {
-        for (uint32_t g = 0; ok && g < units; ++g) ok = qk(g, f);
-      } else {
-        for (uint32_t g = 0; ok && g < units; ++g) ok = pv(g, f, acc);
+        tc_commit(done);  // arrives once every MMA issued above has completed
+        mbar_wait_short(done, 0, a.error_flag);
       }
-      if (elect_one()) tc_commit(done);  // arrives once every MMA issued above has completed
       __syncwarp();
-      wait(done, 0);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ---------------- softmax ----------------
-    constexpr int SC = G_::SC, OC = G_::OC;
+    constexpr int OC = G_::OC;
     const int wg = warp >> 2;
     const int half = NT == 2 ? wg : 0;
     const int r = tid & 127;  // row of the half = TMEM lane
     const uint32_t lane_base = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-    const uint32_t scol = lane_base + G_::s_col(half) + (NT == 1 ? wg * SC : 0);
     const uint32_t ocol = lane_base + G_::o_col(half) + (NT == 1 ? wg * OC : 0);
     const int tk = r / a.G;  // token of the half
     uint32_t g = 0, ga = 0;  // units of this half, and of the CTA
     bool dead = false;
-    auto wait = [&](uint32_t bar, uint32_t parity) {  // voted warp-wide
-      if (!dead) dead = !mbar_wait_warp(bar, parity, a.error_flag);
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      if (!dead) dead = !mbar_wait_short(bar, parity, a.error_flag);
+      __syncwarp();  // the lanes may leave the wait apart, and what follows wants the warp as a whole
     };
-    // P V of this half's unit x is complete.  A barrier tells two phases apart, so each one is waited for in
-    // turn: with P beside S before P's place is written again, with P over S by the S that comes after it.
-    auto wait_o = [&](uint32_t x) {
-      if (NT == 1) wait(odone + 8 * (x & 1), (x >> 1) & 1);
-      else wait(odone + 8 * half, x & 1);
+    // The products so far, up to the part before (unit x, part) of this half, are in O.  A barrier tells two
+    // phases apart; the one before the phase waited for has always been met: by the S that came after it (two
+    // halves), or here, before P's place is written again (one).
+    auto wait_o = [&](uint32_t x, int part) {
+      if (NT == 1) wait(odone + 8 * ((x - 1) & 1), ((x - 1) >> 1) & 1);
+      else if (part == 1) wait(odone + 16 * half, x & 1);
+      else wait(odone + 16 * half + 8, (x - 1) & 1);
+      tc_fence_after();
     };
     auto arrive = [&](uint32_t bar) {  // all lanes' TMEM accesses are ordered before it
       tc_fence_before();
@@ -410,19 +453,26 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
         float m = -INFINITY, l = 0.f;
         bool any = false;     // a unit of the piece has been multiplied
         bool poison = false;  // `mine` holds infinite and NaN values to add to the output
+        bool ready = false;   // every row of the warp has a maximum
         for (int u = 0; u < n; ++u, ++g, ++ga) {
-          wait(sfull + 8 * half, g & 1);
-          tc_fence_after();
-          const bool skip = (meta[ga % kMeta] & kSkip) != 0;
-          const uint32_t pcol = lane_base + G_::p_col(half, g) + (NT == 1 ? wg * 32 : 0);
           const int k0 = t.block_of(c.u + u) * KB;
           const bool whole = attend_whole<KB>(a, t, k0);
-          if (!skip && !whole) {
+#pragma unroll 1
+          for (int part = NT == 1 ? wg : 0; part < 2; part += NT == 1 ? 2 : 1) {  // 64 keys of the block
+          wait(sfull + 16 * half + (NT == 2 ? 8 * part : 0), g & 1);
+          tc_fence_after();
+          const bool skip = (meta[ga % kMeta] & kSkip) != 0;
+          const uint32_t scol = lane_base + G_::s_col(half, part), pcol = lane_base + G_::p_col(half, part, g);
+          uint32_t w[64];  // the row's scores
+          float* s = reinterpret_cast<float*>(w);
+          tmem_ld32_async(scol, w);
+          tmem_ld32_async(scol + 32, w + 32);
+          if (!skip && !whole && (NT == 1 || part == 0)) {
             // A masked key weighs nothing whatever its value row holds, but 0 * inf
             // is not 0 in the product: infinite and NaN values leave the block
             // here and reach the rows that do see them by addition at the end.
             const uint32_t vs = HV * G_::v_at(ga, units);
-            if (NT == 1 && g > 0) wait_o(g - 1);  // its V has been in the slots before this one's
+            if (NT == 1 && g > 0) wait_o(g, 0);  // its V has been in the slots before this one's
 #pragma unroll
             for (int hv = 0; hv < HV; ++hv) wait(full0 + 8 * ((vs + hv) % S), ((vs + hv) / S) & 1);
             bool odd = false;
@@ -473,43 +523,44 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
               named_sync(team);
             }
           }
+          tmem_ld_wait();
+          tmem_ready32(w);
+          tmem_ready32(w + 32);
+          if (NT == 1) {
+            arrive(sread);
+            if (g > 1) wait_o(g - 1, 0);  // the unit before the last has left P's place
+          }
           if (!skip) {
-            uint32_t w[SC];
-            float* s = reinterpret_cast<float*>(w);
-            const int c0 = k0 + (NT == 1 ? wg * SC : 0);  // attend_sees, relative to the row's columns
-            const int hi = pos - c0, lo = a.window > 0 ? hi - a.window : -1, first = a.sinks - c0;
-            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            tmem_ld32_async(scol, w);
+            // weights of the 64 keys, rounded into p; returns the sum of the unrounded ones
+            uint32_t p[32];
+            auto weigh = [&]() {
+              const float ms = m == -INFINITY ? 0.f : m * a.scale_log2;
+              const float2 c2 = make_float2(a.scale_log2, a.scale_log2), n2 = make_float2(-ms, -ms);
+              float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-            for (int i = 0; i < SC; i += 32) {  // the next 32 columns are on their way under the maximum of these
-              tmem_ld_wait();
-              tmem_ready32(w + i);
-              if (i + 32 < SC) tmem_ld32_async(scol + i + 32, w + i + 32);
-              if (!whole) {
-#pragma unroll
-                for (int j = i; j < i + 32; ++j) s[j] = j <= hi && (j > lo || j < first) ? s[j] : -INFINITY;
+              for (int j = 0; j < 32; ++j) {
+                const float2 x = __ffma2_rn(make_float2(s[2 * j], s[2 * j + 1]), c2, n2);
+                const float2 e = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+                sum[j & 1] = __fadd2_rn(sum[j & 1], e);
+                p[j] = pack<FP16>(e.x, e.y);
               }
+              sum[0] = __fadd2_rn(sum[0], sum[1]);
+              return sum[0].x + sum[0].y;
+            };
+            auto largest = [&]() {
+              float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-              for (int j = i; j < i + 32; j += 8)
+              for (int j = 4; j < 60; j += 8)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) top[k] = max3(top[k], s[j + k], s[j + 4 + k]);
-            }
-            if constexpr (G_::kBeside) arrive(sread + 8 * half);
-            float mx = max3(fmaxf(top[0], top[1]), top[2], top[3]);
-            if constexpr (NT == 1) {
-              xch[((g & 1) * 2 + wg) * 128 + r] = mx;
-              tc_fence_before();
-              named_sync(256);  // and both halves of S are read: P may overwrite them
-              tc_fence_after();
-              mx = fmaxf(mx, xch[((g & 1) * 2 + (wg ^ 1)) * 128 + r]);
-            }
-            const bool raise = m > -INFINITY && mx * a.scale_log2 > m * a.scale_log2 + kSlack;
-            if (__any_sync(0xffffffffu, raise)) {  // rescale the output and the sum
-              const float f = raise ? exp2_approx((m - mx) * a.scale_log2) : 1.f;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) top[k] = fmaxf(top[k], s[60 + k]);
+              return max3(fmaxf(top[0], top[1]), top[2], top[3]);
+            };
+            // a new maximum: the row's sum and its output so far times f
+            auto rescale = [&](float f) {
               l *= f;
-              if (raise) m = mx;
-              wait_o(g - 1);  // the output so far
-              tc_fence_after();
+              wait_o(g, NT == 1 ? 0 : part);
 #pragma unroll 1
               for (int i = 0; i < OC; i += 32) {
                 uint32_t o[32];
@@ -518,38 +569,42 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
                 for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
                 tmem_st32(ocol + i, o);
               }
+            };
+            float sum = 0.f;
+            // The weights are taken with the maximum as it stands, and only a sum that is too large (or a row's
+            // first keys) asks for the scores' own: no pass for the maximum in most blocks.
+            bool fine = false;
+            if (NT == 2 && whole && ready) {
+              sum = weigh();
+              fine = __all_sync(0xffffffffu, !live || sum <= kMost);
             }
-            if (m == -INFINITY) m = mx;  // nothing seen so far: l and the output row are 0
-            const float ms = m == -INFINITY ? 0.f : m * a.scale_log2;
-            if (G_::kBeside && g > NT % 2) {  // what P's place held has been read
-              wait_o(g - (NT == 1 ? 2 : 1));
-              tc_fence_after();
-            }
-            const float2 c2 = make_float2(a.scale_log2, a.scale_log2), n2 = make_float2(-ms, -ms);
-            float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            if (__builtin_expect(!fine, 0)) {
+              if (!whole) {
+                const int c0 = k0 + 64 * part;  // attend_sees, relative to the row's columns
+                const int hi = pos - c0, lo = a.window > 0 ? hi - a.window : -1, first = a.sinks - c0;
 #pragma unroll
-            for (int i = 0; i < SC; i += 32) {
-              uint32_t p[16];
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                const float2 x = __ffma2_rn(make_float2(s[i + 2 * j], s[i + 2 * j + 1]), c2, n2);
-                const float2 e = make_float2(exp2_approx(x.x), exp2_approx(x.y));
-                sum[j & 1] = __fadd2_rn(sum[j & 1], e);
-                p[j] = pack<FP16>(e.x, e.y);
+                for (int j = 0; j < 64; ++j) s[j] = j <= hi && (j > lo || j < first) ? s[j] : -INFINITY;
               }
-              tmem_st16(pcol + i / 2, p);
-              if (i % 64 == 32) {
-                tc_wait_st();
-                arrive(pfull + 16 * half + 8 * (NT == 1 ? wg : i / 64));
+              float mx = largest();
+              if constexpr (NT == 1) {
+                xch[((g & 1) * 2 + wg) * 128 + r] = mx;
+                named_sync(256);
+                mx = fmaxf(mx, xch[((g & 1) * 2 + (wg ^ 1)) * 128 + r]);
               }
+              const bool raise = !(mx <= m) && (m == -INFINITY || !((mx - m) * a.scale_log2 <= kSlack));  // or NaN
+              const float f = raise && m > -INFINITY ? exp2_approx((m - mx) * a.scale_log2) : 1.f;
+              if (raise) m = mx;
+              if (__any_sync(0xffffffffu, f != 1.f)) rescale(f);
+              sum = weigh();
+              if (live && !(sum <= kMost)) sum = NAN;  // a score is infinite or NaN
+              ready = __all_sync(0xffffffffu, !live || m > -INFINITY);
             }
-            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+            l += sum;
             any = true;
-          } else {
-            if (G_::kBeside && g > NT % 2) wait_o(g - (NT == 1 ? 2 : 1));
-            if constexpr (G_::kBeside) arrive(sread + 8 * half);
-            if (NT == 2 || wg == 0) arrive(pfull + 16 * half);
-            if (NT == 2 || wg == 1) arrive(pfull + 16 * half + 8);
+            tmem_st32(pcol, p);
+            tc_wait_st();
+          }
+          arrive(pfull + 16 * half + 8 * part);
           }
         }
         // ---- the piece's output ----
@@ -560,10 +615,10 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
           l += xch[(wg ^ 1) * 128 + r];
           named_sync(256);
         }
-        wait_o(g - 1);
-        tc_fence_after();
+        wait_o(g, 0);
         const int head = c.h * a.G + r - tk * a.G;
-        const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing answers 0
+        if (m == -INFINITY) any = false, l = 0.f;  // a row that has seen nothing answers 0
+        const float inv = l == 0.f ? 0.f : 1.f / l;
         uint16_t* dst = a.out + (int64_t)(t.row0 + token) * a.o_tok + (int64_t)head * a.o_head + (NT == 1 ? wg * OC : 0);
 #pragma unroll 1
         for (int i = 0; i < OC; i += 32) {
@@ -598,7 +653,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
         if (live && (NT == 2 || wg == 0)) {
           if (!(starts && ends)) a.part_ml[part * a.rows + token * a.G + r - tk * a.G] = make_float2(m, l);
           else if (a.lse)
-            a.lse[(int64_t)(t.row0 + token) * a.Hq + head] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
+            a.lse[(int64_t)(t.row0 + token) * a.Hq + head] = m == -INFINITY ? -INFINITY : m * a.scale + logf(l);
         }
         arrive(ofree + 8 * half);
       } else {

@@ -19,10 +19,7 @@ __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence:
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// One lane of the warp, always the same, as the compiler can tell: tcgen05.mma
-// takes its descriptors from uniform registers, and under a plain
-// `if (lane == 0)` each one is moved there lane by lane (about 200 cycles an
-// instruction, against the 64 that a 128 x 128 x 16 product takes).
+// One lane of the warp, always the same one.
 __device__ __forceinline__ bool elect_one() {
   uint32_t y;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(y)::"memory");
