@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_rows_kernel(const __grid_c
       if (!dead && k0 >= 0) {
         const uint32_t kt = stage0 + s * G_::kStage, vt = kt + G_::kTile;
         const int w0 = warp * NK;  // this warp's keys of the block
-        const bool whole = attend_whole<KB>(a, t, k0);
+        const bool whole = attend_whole(a, t.pos0, t.last(), k0, KB);
         float x[NK / 8][4];
 #pragma unroll
         for (int i = 0; i < NK / 8; ++i) x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;

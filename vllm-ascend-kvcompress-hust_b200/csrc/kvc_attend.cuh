@@ -217,11 +217,10 @@ __device__ __forceinline__ void attend_advance(const AttendArgs& a, AttendCursor
   } while (attend_tiles(a, c.r) == 0);
 }
 
-// whether every row of the tile sees all KB keys from k0 on
-template <int KB>
-__device__ __forceinline__ bool attend_whole(const AttendArgs& a, const AttendTile& t, int k0) {
-  if (k0 + KB - 1 > t.pos0) return false;
-  return a.window == 0 || k0 > t.last() - a.window || k0 + KB <= a.sinks;
+// whether rows at positions first to last see all n keys from k0 on
+__device__ __forceinline__ bool attend_whole(const AttendArgs& a, int first, int last, int k0, int n) {
+  if (k0 + n - 1 > first) return false;
+  return a.window == 0 || k0 > last - a.window || k0 + n <= a.sinks;
 }
 
 __device__ __forceinline__ bool attend_sees(const AttendArgs& a, int pos, int key) {

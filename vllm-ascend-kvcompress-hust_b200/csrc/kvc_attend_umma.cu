@@ -109,13 +109,13 @@ __device__ __forceinline__ void tma_4d(uint32_t dst, const void* map, int c0, in
 __device__ __forceinline__ void named_sync(int threads) {
   asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");
 }
-__device__ __forceinline__ bool named_or(int threads, bool x) {
+__device__ __forceinline__ bool named_or(int id, int threads, bool x) {
   uint32_t y;
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 2, %2, p;\n\t"
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %3, %2, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(y)
-      : "r"((uint32_t)x), "r"(threads)
+      : "r"((uint32_t)x), "r"(threads), "r"(id)
       : "memory");
   return y != 0;
 }
@@ -449,14 +449,15 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
         const int pos = live ? t.pos0 + token : -1;
         const int64_t part = 2 * (int64_t)blockIdx.x + (starts ? 1 : 0);
         float* mine = a.part_o + (part * a.rows + (int64_t)token * a.G + r - tk * a.G) * D + (NT == 1 ? wg * OC : 0);
-        const int team = NT == 1 ? 256 : 128 * halves;  // threads that look at a V block together
+        // positions of this half's rows
+        const int pos_first = t.pos0 + half * a.sub, pos_last = min(t.last(), pos_first + a.sub - 1);
         float m = -INFINITY, l = 0.f;
         bool any = false;     // a unit of the piece has been multiplied
         bool poison = false;  // `mine` holds infinite and NaN values to add to the output
         bool ready = false;   // every row of the warp has a maximum
         for (int u = 0; u < n; ++u, ++g, ++ga) {
           const int k0 = t.block_of(c.u + u) * KB;
-          const bool whole = attend_whole<KB>(a, t, k0);
+          const bool whole = attend_whole(a, t.pos0, t.last(), k0, KB);  // for the tile
 #pragma unroll 1
           for (int part = NT == 1 ? wg : 0; part < 2; part += NT == 1 ? 2 : 1) {  // 64 keys of the block
           wait(sfull + 16 * half + (NT == 2 ? 8 * part : 0), g & 1);
@@ -478,13 +479,16 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
             bool odd = false;
             constexpr int kVec = KB * D / 8;
             auto vaddr = [&](int i) { return ring0 + ((vs + i / (SK * D / 8)) % S) * G_::kSlot + (i % (SK * D / 8)) * 16; };
-            const int me = team == 256 ? tid : r;
-            for (int i = me; i < kVec; i += team) {
+            // Each warpgroup looks for itself (with one half they share the block), and nothing is cleared
+            // before both have looked, so both find the same.
+            constexpr int kLook = NT == 1 ? 256 : 128;
+            for (int i = tid % kLook; i < kVec; i += kLook) {
               uint32_t w[4];
               lds128(vaddr(i), w);
               odd |= odd_pair<FP16>(w[0]) | odd_pair<FP16>(w[1]) | odd_pair<FP16>(w[2]) | odd_pair<FP16>(w[3]);
             }
-            if (named_or(team, odd)) {
+            const int team = NT == 1 || halves == 2 ? 256 : 128;
+            if (named_or(2 + (NT == 1 ? 0 : wg), kLook, odd)) {
               const int d0 = NT == 1 ? wg * OC : 0;
               if (live && !poison) {
                 for (int d = 0; d < OC; ++d) mine[d] = 0.f;
@@ -507,7 +511,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
                 }
               }
               named_sync(team);  // read by all before it is cleared
-              for (int i = me; i < kVec; i += team) {
+              for (int i = team == 256 ? tid : r; i < kVec; i += team) {
                 const uint32_t ad = vaddr(i);
                 uint32_t w[4];
                 lds128(ad, w);
@@ -574,12 +578,13 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
             // The weights are taken with the maximum as it stands, and only a sum that is too large (or a row's
             // first keys) asks for the scores' own: no pass for the maximum in most blocks.
             bool fine = false;
-            if (NT == 2 && whole && ready) {
+            const bool seen = whole || attend_whole(a, pos_first, pos_last, k0 + 64 * part, 64);  // by this half's rows
+            if (NT == 2 && seen && ready) {
               sum = weigh();
               fine = __all_sync(0xffffffffu, !live || sum <= kMost);
             }
             if (__builtin_expect(!fine, 0)) {
-              if (!whole) {
+              if (!seen) {
                 const int c0 = k0 + 64 * part;  // attend_sees, relative to the row's columns
                 const int hi = pos - c0, lo = a.window > 0 ? hi - a.window : -1, first = a.sinks - c0;
 #pragma unroll
