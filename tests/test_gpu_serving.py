@@ -113,7 +113,8 @@ def check_rotary(c, q_got, kc_got, vc_got, slots):
 
 @pytest.mark.parametrize("n,heads,kvh,dim,rot,axes,dtype,far", [
     (1, 5, 1, 128, 128, 1, BF16, 100), (37, 16, 2, 256, 64, 3, BF16, 52000), (130, 8, 8, 64, 64, 1, FP16, 1 << 20),
-    (300, 20, 4, 128, 64, 4, FP16, 40000), (9, 3, 1, 72, 48, 2, BF16, 1 << 40), (5, 2, 2, 256, 256, 1, BF16, 7)])
+    (300, 20, 4, 128, 64, 4, FP16, 40000), (9, 3, 1, 72, 48, 2, BF16, 1 << 40), (5, 2, 2, 256, 256, 1, BF16, 7),
+    (3, 2, 1, 16, 16, 1, FP16, 50), (2371, 3, 1, 64, 32, 3, BF16, 9000), (4000, 2, 2, 16, 16, 1, BF16, 70000)])
 def test_rotary_write(n, heads, kvh, dim, rot, axes, dtype, far):
     c = rotary_case(n, heads, kvh, dim, rot, axes, dtype, far)
     if n > 4:

@@ -10,12 +10,16 @@
 // Bound: HBM, 4 bytes per element of q, k and v (one read, one write), so q, k
 // and v are touched once, in 16-byte vectors, and the rotated keys never exist
 // outside the cache.  The angles are formed here rather than read from a
-// table: a token's F angles serve its (q + kv) heads, so one CTA per token
-// computes them once into shared memory.  An angle of a far position loses
-// fp32's bits (position 50,000 at omega = 1 would be off by 2e-3), so the
-// product and its reduction to (-1, 1] half turns are taken in fp64, which is
-// F products per token next to 2 (q + 2 kv) D bytes of traffic; sine and cosine
-// of the reduced angle, and the rotation, are fp32, rounded once to 16 bits.
+// table: a token's F angles serve its (q + kv) heads, so a CTA computes them
+// once into shared memory.  An angle of a far position loses fp32's bits
+// (position 50,000 at omega = 1 would be off by 2e-3), so the product and its
+// reduction to (-1, 1] half turns are taken in fp64, which is F products per
+// token next to 2 (q + 2 kv) D bytes of traffic; sine and cosine of the reduced
+// angle, and the rotation, are fp32, rounded once to 16 bits.
+//
+// Four tokens a CTA once there are enough of them to fill the GPU several times
+// (8,191 tokens, 16 q and 2 kv heads of 256 dims, 64 of them turned: 34.5 us, 4.9
+// TB/s; 2 tokens 39, 8 tokens 44, one token 42 us), else one, for latency.
 #include <algorithm>
 #include <type_traits>
 
@@ -25,6 +29,7 @@ namespace {
 
 constexpr int kMaxFreq = 128;
 constexpr int kMaxAxes = 8;
+constexpr int kThreads = 128, kTokens = 4;
 
 struct RotaryArgs {
   const uint16_t* q;
@@ -40,8 +45,9 @@ struct RotaryArgs {
   int32_t* error_flag;
   int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head, o_tok, o_head;  // strides in elements
   int64_t pos_stride, k_block, v_block;                                // block strides in elements
-  int64_t num_slots;
+  int64_t num_slots, num_tokens;
   int Hq, Hk, D, F, axes;
+  uint32_t per_magic, vec_magic;  // ceil(2^32 / vectors of a q or k head), and of a v head
   bool in_place;  // q_out is q: the pass band is already there
 };
 
@@ -69,57 +75,94 @@ __device__ __forceinline__ void rotate8(uint4& x, uint4& y, const float* cs, con
   y = make_uint4(yw[0], yw[1], yw[2], yw[3]);
 }
 
-template <class E>
-__global__ void __launch_bounds__(256) rotary_write_kernel(const __grid_constant__ RotaryArgs a) {
+// A token's work in 16-byte pieces: of each q and k head first the F / 8 pairs of
+// vectors that turn into each other, then the passing ones; then the v heads.
+// A CTA takes T tokens: a thread works out where its piece lies once for all of
+// them, has their T (or 2 T) loads on their way at once, the first ones while
+// the angles are formed, and the T F angles keep every thread busy.
+template <class E, int T>
+__global__ void __launch_bounds__(kThreads) rotary_write_kernel(const __grid_constant__ RotaryArgs a) {
   kvc::pdl_wait();
   kvc::pdl_trigger();
-  __shared__ __align__(16) float cs[kMaxFreq], sn[kMaxFreq];
-  const int64_t t = blockIdx.x;
-  const int tid = threadIdx.x, nt = blockDim.x;
-  for (int f = tid; f < a.F; f += nt) {
-    int ax = a.axis ? __ldg(a.axis + f) : 0;
-    if (ax < 0 || ax >= a.axes) {
-      kvc::raise_flag(a.error_flag, KVC_DEV_INDEX_RANGE);
-      ax = 0;
+  __shared__ __align__(16) float cs[T][kMaxFreq], sn[T][kMaxFreq];
+  const int64_t t0 = (int64_t)blockIdx.x * T;
+  const int n = T == 1 ? 1 : (int)kvc::min64(T, a.num_tokens - t0);
+  const int tid = threadIdx.x;
+  const int pairs = a.F / 8, per = pairs + (a.D - 2 * a.F) / 8, vec = a.D / 8;
+  const int turned = (a.Hq + a.Hk) * per, items = turned + a.Hk * vec;
+  __shared__ int64_t place[2][T];  // of the tokens' rows in the K and V caches, or -1
+  bool angles = false;
+  for (int base = 0; base < items; base += kThreads) {
+    const int i = base + tid;
+    const bool mine = i < items, value = i >= turned;
+    const int k = value ? i - turned : i, of = value ? vec : per;
+    const int h = of == 1 ? k : (int)__umulhi((uint32_t)k, value ? a.vec_magic : a.per_magic);
+    const bool key = !value && h >= a.Hq, query = !value && !key;
+    const bool pair = !value && k - h * of < pairs;
+    const int dim = 8 * (k - h * of) + (value || pair ? 0 : a.F);  // 2 F + 8 (j - pairs) past the pairs
+    const uint16_t* src = value ? a.v + t0 * a.v_tok + h * a.v_head
+                          : key ? a.k + t0 * a.k_tok + (h - a.Hq) * a.k_head
+                                : a.q + t0 * a.q_tok + h * a.q_head;
+    const int64_t step = value ? a.v_tok : key ? a.k_tok : a.q_tok;
+    uint4 x[T], y[T];
+    if (mine) {
+#pragma unroll
+      for (int j = 0; j < T; ++j)
+        if (j < n) {
+          x[j] = load16(src + j * step + dim);
+          if (pair) y[j] = load16(src + j * step + dim + a.F);
+        }
     }
-    // half turns, reduced to [-1, 1]
-    const double u = (double)__ldg(a.positions + ax * a.pos_stride + t) * (double)__ldg(a.omega + f) *
-                     0.31830988618379067154;
-    sincospif((float)(u - 2.0 * rint(0.5 * u)), &sn[f], &cs[f]);
+    if (!angles) {
+      angles = true;
+      if (tid < T) {
+        int64_t slot = tid < n ? __ldg(a.slots + t0 + tid) : -1;
+        if (slot >= a.num_slots) {
+          kvc::raise_flag(a.error_flag, KVC_DEV_TOKEN_RANGE);
+          slot = -1;
+        }
+        const int64_t block = slot / kvc::kBlock, row = (slot % kvc::kBlock) * a.Hk * a.D;
+        place[0][tid] = slot < 0 ? -1 : block * a.k_block + row;
+        place[1][tid] = slot < 0 ? -1 : block * a.v_block + row;
+      }
+      for (int e = tid; e < n * a.F; e += kThreads) {
+        const int j = T == 1 ? 0 : e / a.F, f = e - j * a.F;
+        int ax = a.axis ? __ldg(a.axis + f) : 0;
+        if (ax < 0 || ax >= a.axes) {
+          kvc::raise_flag(a.error_flag, KVC_DEV_INDEX_RANGE);
+          ax = 0;
+        }
+        // half turns, reduced to [-1, 1]
+        const double u = (double)__ldg(a.positions + ax * a.pos_stride + t0 + j) * (double)__ldg(a.omega + f) *
+                         0.31830988618379067154;
+        sincospif((float)(u - 2.0 * rint(0.5 * u)), &sn[j][f], &cs[j][f]);
+      }
+      __syncthreads();
+    }
+    if (!mine || (query && !pair && a.in_place)) continue;
+    uint16_t* to = query ? a.q_out + t0 * a.o_tok + h * a.o_head + dim
+                   : value ? a.v_cache + h * a.D + dim
+                           : a.k_cache + (h - a.Hq) * a.D + dim;
+#pragma unroll
+    for (int j = 0; j < T; ++j) {
+      if (j >= n) continue;
+      const int64_t off = query ? j * a.o_tok : place[value][j];
+      if (off < 0) continue;
+      uint16_t* dst = to + off;
+      if (pair) {
+        rotate8<E>(x[j], y[j], cs[j] + dim, sn[j] + dim);
+        *reinterpret_cast<uint4*>(dst + a.F) = y[j];
+      }
+      *reinterpret_cast<uint4*>(dst) = x[j];
+    }
   }
-  int64_t slot = __ldg(a.slots + t);
-  if (slot >= a.num_slots) {
-    if (tid == 0) kvc::raise_flag(a.error_flag, KVC_DEV_TOKEN_RANGE);
-    slot = -1;
-  }
-  const int64_t block = slot / kvc::kBlock, row = (slot % kvc::kBlock) * a.Hk;
-  uint16_t* kd = a.k_cache + block * a.k_block + row * a.D;
-  uint16_t* vd = a.v_cache + block * a.v_block + row * a.D;
-  __syncthreads();
+}
 
-  const int pairs = a.F / 8, pass = (a.D - 2 * a.F) / 8, per = pairs + pass;
-  const int heads = slot < 0 ? a.Hq : a.Hq + a.Hk;  // a token without a slot turns its queries alone
-  for (int i = tid; i < heads * per; i += nt) {
-    const int h = i / per, j = i - h * per;
-    const bool key = h >= a.Hq;
-    const uint16_t* src = key ? a.k + t * a.k_tok + (h - a.Hq) * a.k_head : a.q + t * a.q_tok + h * a.q_head;
-    uint16_t* dst = key ? kd + (h - a.Hq) * a.D : a.q_out + t * a.o_tok + h * a.o_head;
-    if (j < pairs) {
-      uint4 x = load16(src + 8 * j), y = load16(src + a.F + 8 * j);
-      rotate8<E>(x, y, cs + 8 * j, sn + 8 * j);
-      *reinterpret_cast<uint4*>(dst + 8 * j) = x;
-      *reinterpret_cast<uint4*>(dst + a.F + 8 * j) = y;
-    } else if (key || !a.in_place) {
-      const int d = 2 * a.F + 8 * (j - pairs);
-      *reinterpret_cast<uint4*>(dst + d) = load16(src + d);
-    }
-  }
-  if (slot < 0) return;
-  const int vec = a.D / 8;
-  for (int i = tid; i < a.Hk * vec; i += nt) {
-    const int h = i / vec, d = (i - h * vec) * 8;
-    *reinterpret_cast<uint4*>(vd + h * a.D + d) = load16(a.v + t * a.v_tok + h * a.v_head + d);
-  }
+template <int T>
+void launch(const RotaryArgs& a, bool bf16, cudaStream_t st) {
+  const dim3 grid((unsigned)((a.num_tokens + T - 1) / T)), block(kThreads);
+  if (bf16) kvc::launch_dep(rotary_write_kernel<kvc::Bf16, T>, grid, block, 0, st, a);
+  else kvc::launch_dep(rotary_write_kernel<kvc::Fp16, T>, grid, block, 0, st, a);
 }
 
 }  // namespace
@@ -136,7 +179,9 @@ extern "C" int kvc_rotary_write(const void* q, int64_t q_token_stride, int64_t q
                     (dtype == KVC_BF16 || dtype == KVC_FP16) && axes >= 1 && axes <= kMaxAxes && head_dim > 0 &&
                     rotary_dim > 0 && rotary_dim <= head_dim && position_stride >= 0,
                 KVC_EINVAL);
-  KVC_CHECK_ARG(head_dim % 8 == 0 && rotary_dim % 16 == 0 && rotary_dim / 2 <= kMaxFreq, KVC_EUNSUPPORTED);
+  KVC_CHECK_ARG(head_dim % 8 == 0 && rotary_dim % 16 == 0 && rotary_dim / 2 <= kMaxFreq && head_dim <= 1024 &&
+                    heads <= 4096 && kv_heads <= 4096,
+                KVC_EUNSUPPORTED);
   if (num_tokens == 0) return KVC_OK;
   KVC_CHECK_ARG(q && k && v && positions && omega && slot_mapping && q_out && k_cache && v_cache, KVC_ENULL);
   KVC_CHECK_ARG(axes == 1 || axis_of_frequency, KVC_ENULL);
@@ -168,10 +213,11 @@ extern "C" int kvc_rotary_write(const void* q, int64_t q_token_stride, int64_t q
   a.num_slots = num_blocks * kvc::kBlock;
   a.Hq = heads, a.Hk = kv_heads, a.D = head_dim, a.F = rotary_dim / 2, a.axes = axes;
   a.in_place = q_out == q && out_token_stride == q_token_stride && out_head_stride == q_head_stride;
-  const dim3 grid((unsigned)num_tokens), block(128);
-  if (dtype == KVC_BF16)
-    kvc::launch_dep(rotary_write_kernel<kvc::Bf16>, grid, block, 0, (cudaStream_t)stream, a);
-  else
-    kvc::launch_dep(rotary_write_kernel<kvc::Fp16>, grid, block, 0, (cudaStream_t)stream, a);
+  const auto magic = [](int n) { return (uint32_t)(((1ull << 32) + n - 1) / n); };  // exact for i * n < 2^32, n > 1
+  a.per_magic = magic(rotary_dim / 16 + (head_dim - rotary_dim) / 8);
+  a.vec_magic = magic(head_dim / 8);
+  a.num_tokens = num_tokens;
+  if (num_tokens >= kTokens * 4 * kvc::sm_count()) launch<kTokens>(a, dtype == KVC_BF16, (cudaStream_t)stream);
+  else launch<1>(a, dtype == KVC_BF16, (cudaStream_t)stream);
   return kvc::launch_status();
 }
