@@ -398,48 +398,72 @@ int launch_t(const AttendArgs& a, cudaStream_t st) {
 
 constexpr int kCombineWarps = 4;
 
-// blockIdx.x: the CTA in which the tile starts; warps of blockIdx.y share the rows.
-template <bool FP16>
+// blockIdx.x: the CTA in which the tile starts; the warps of blockIdx.y share the rows.  Four parts at a time
+// are on their way with their (m, l), and joined with a running maximum, so that nothing but the record comes
+// before the loads: 250 rows of 128 values in 2 to 3 parts for each of 148 CTAs, 40 MB.
+template <int D, bool FP16>
 __global__ void __launch_bounds__(kCombineWarps * 32) attend_combine_kernel(const __grid_constant__ AttendArgs a) {
   pdl_wait();
   pdl_trigger();
+  constexpr int kLanes = D < 128 ? D / 4 : 32;  // of a row, 4 values each, kVec times
+  constexpr int kVec = D / (4 * kLanes), kRowsAtOnce = 32 / kLanes, kParts = 4;
   const int4 rec = a.record[blockIdx.x];
   if (rec.x == 0) return;
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, in_row = lane % kLanes;
   const int rows = rec.z * a.G, parts = rec.x + 1;
   const int64_t first = 2 * (int64_t)blockIdx.x;  // part 0 is slot first + 1, part j slot first + 2 j
-  auto slot = [&](int j) { return j == 0 ? first + 1 : first + 2 * (int64_t)j; };
-  for (int row = blockIdx.y * kCombineWarps + (threadIdx.x >> 5); row < rows; row += gridDim.y * kCombineWarps) {
-    float mx = -INFINITY;
-    for (int j = lane; j < parts; j += 32) mx = fmaxf(mx, a.part_ml[slot(j) * a.rows + row].x);
+  for (int row = (blockIdx.y * kCombineWarps + (threadIdx.x >> 5)) * kRowsAtOnce + lane / kLanes; row < rows;
+       row += gridDim.y * kCombineWarps * kRowsAtOnce) {
+    float m = -INFINITY, sum = 0.f;
+    float4 acc[kVec];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    const int tk = row / a.G, head = rec.w * a.G + row - tk * a.G;
-    for (int d0 = 0; d0 < a.D; d0 += 128) {
-      const int d = d0 + 4 * lane;
-      float sum = 0.f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int j = 0; j < parts; ++j) {  // in unit order
-        const int64_t at = slot(j) * a.rows + row;
-        const float2 ml = a.part_ml[at];
-        const float f = ml.x == -INFINITY ? 1.f : exp2_approx((ml.x - mx) * a.scale_log2);
-        sum += f * ml.y;
-        if (d < a.D) {
-          const float4 v = *reinterpret_cast<const float4*>(a.part_o + at * a.D + d);
-          acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
+    for (int i = 0; i < kVec; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j0 = 0; j0 < parts; j0 += kParts) {  // in unit order
+      float2 ml[kParts];
+      float4 v[kParts][kVec];
+#pragma unroll
+      for (int j = 0; j < kParts; ++j) {
+        ml[j] = make_float2(-INFINITY, 0.f);
+        if (j0 + j >= parts) continue;
+        const int64_t at = (j0 + j == 0 ? first + 1 : first + 2 * (int64_t)(j0 + j)) * a.rows + row;
+        ml[j] = a.part_ml[at];
+#pragma unroll
+        for (int i = 0; i < kVec; ++i)
+          v[j][i] = *reinterpret_cast<const float4*>(a.part_o + at * D + 4 * (in_row + i * kLanes));
+      }
+      float mx = m;
+#pragma unroll
+      for (int j = 0; j < kParts; ++j) mx = fmaxf(mx, ml[j].x);
+      // an empty part has o = l = 0, or, with values that are not finite, what it has to add
+      const float keep = m == -INFINITY ? 1.f : exp2_approx((m - mx) * a.scale_log2);
+      m = mx;
+      sum *= keep;
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) acc[i].x *= keep, acc[i].y *= keep, acc[i].z *= keep, acc[i].w *= keep;
+#pragma unroll
+      for (int j = 0; j < kParts; ++j) {
+        if (j0 + j >= parts) continue;
+        const float f = ml[j].x == -INFINITY ? 1.f : exp2_approx((ml[j].x - mx) * a.scale_log2);
+        sum += f * ml[j].y;
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+          acc[i].x += f * v[j][i].x, acc[i].y += f * v[j][i].y;
+          acc[i].z += f * v[j][i].z, acc[i].w += f * v[j][i].w;
         }
       }
-      if (d < a.D) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        uint2 w;
-        w.x = pack<FP16>(acc.x * inv, acc.y * inv);
-        w.y = pack<FP16>(acc.z * inv, acc.w * inv);
-        *reinterpret_cast<uint2*>(a.out + (int64_t)(rec.y + tk) * a.o_tok + (int64_t)head * a.o_head + d) = w;
-      }
-      if (a.lse && d == 0)
-        a.lse[(int64_t)(rec.y + tk) * a.Hq + head] = sum == 0.f ? -INFINITY : mx * a.scale + logf(sum);
     }
+    const int tk = row / a.G, head = rec.w * a.G + row - tk * a.G;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing answers 0
+    uint16_t* dst = a.out + (int64_t)(rec.y + tk) * a.o_tok + (int64_t)head * a.o_head;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      uint2 w;
+      w.x = pack<FP16>(acc[i].x * inv, acc[i].y * inv);
+      w.y = pack<FP16>(acc[i].z * inv, acc[i].w * inv);
+      *reinterpret_cast<uint2*>(dst + 4 * (in_row + i * kLanes)) = w;
+    }
+    if (a.lse && in_row == 0)
+      a.lse[(int64_t)(rec.y + tk) * a.Hq + head] = sum == 0.f ? -INFINITY : m * a.scale + logf(sum);
   }
 }
 
@@ -450,9 +474,12 @@ int rows_launch(const AttendArgs& a, bool fp16, cudaStream_t st) {
 }
 
 int combine_launch(const AttendArgs& a, bool fp16, cudaStream_t st) {
-  const unsigned y = (unsigned)((a.rows + 2 * kCombineWarps - 1) / (2 * kCombineWarps));
-  if (fp16) launch_dep(attend_combine_kernel<true>, dim3((unsigned)a.ctas, y), dim3(kCombineWarps * 32), 0, st, a);
-  else launch_dep(attend_combine_kernel<false>, dim3((unsigned)a.ctas, y), dim3(kCombineWarps * 32), 0, st, a);
+  const unsigned y = (unsigned)a.rows / (a.rows > kRows ? 16 : 8);
+  const dim3 grid((unsigned)a.ctas, y), block(kCombineWarps * 32);
+  if (a.D == 64) launch_dep(fp16 ? attend_combine_kernel<64, true> : attend_combine_kernel<64, false>, grid, block, 0, st, a);
+  else if (a.D == 128)
+    launch_dep(fp16 ? attend_combine_kernel<128, true> : attend_combine_kernel<128, false>, grid, block, 0, st, a);
+  else launch_dep(fp16 ? attend_combine_kernel<256, true> : attend_combine_kernel<256, false>, grid, block, 0, st, a);
   return launch_status();
 }
 
