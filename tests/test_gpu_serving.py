@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import math
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -10,6 +11,7 @@ import torch
 import serving_reference as R
 from vllm_ascend_kvcompress import _native as N
 from vllm_ascend_kvcompress.methods.triattention import kernels as K
+from vllm_ascend_kvcompress.provider import ActiveCompression, BatchedCompressionProvider
 
 pytestmark = pytest.mark.gpu
 BF16, FP16 = torch.bfloat16, torch.float16
@@ -401,3 +403,124 @@ def test_a_step_over_a_compressed_cache(scheduled):
     assert torch.equal(gv.flatten(0, 1)[slots], hv)
     c = {"q": q.cpu(), "kc": gk, "vc": gv, "table": torch.tensor(want[5]), "starts": want[0], "lens": want[1]}
     check_attention(c, got)
+
+
+def test_the_provider_makes_the_tables_of_its_batch():
+    ids = ["a", "b", "c"]
+    runner = SimpleNamespace(device=torch.device("cuda"), requests={r: None for r in ids}, max_num_reqs=4,
+                             max_num_tokens=64, input_batch=SimpleNamespace(req_ids=ids, num_reqs=3))
+    p = BatchedCompressionProvider(SimpleNamespace(runtime_spec=None), runner, scheduler_block_size=256)
+    p.active["b"] = ActiveCompression(5000, 300)
+    p.after_update_states(None)
+    pages = torch.arange(30).view(3, 10)
+    t = p.step_tables(ints([10, 5003, 700]), ints([4, 1, 1]), pages.cuda(), num_tokens=6, max_blocks=6)
+    check_tables(t, R.step_tables([10, 5003, 700], [4, 1, 1], [0, 4700, 0], pages.tolist(), 2, 6, 6))
+    p.check_device_errors()
+    p.step_tables(ints([10, 5003, 9000]), ints([4, 1, 1]), pages.cuda(), num_tokens=6, max_blocks=6)
+    with pytest.raises(RuntimeError, match="step_tables"):
+        p.check_device_errors()
+    with pytest.raises(RuntimeError, match="max_num_reqs"):
+        p.step_tables(ints([1] * 5), ints([1] * 5), pages.cuda(), num_tokens=5, max_blocks=1)
+
+
+# ---- refusals of the wrappers ---------------------------------------------------------------------
+
+
+def test_wrappers_refuse_what_does_not_fit():
+    i32 = ints([3, 4])
+    pages = ints([[0, 1], [2, 3]])
+    for bad in (dict(offsets=i32), dict(max_blocks=-1), dict(num_tokens=-1), dict(blocks_per_page=0)):
+        with pytest.raises((RuntimeError, ValueError)):
+            K.step_tables(i32, i32, pages, **{"num_tokens": 7, "max_blocks": 1, **bad})
+    for bad in ((i32[:1], i32, pages), (i32.float(), i32, pages), (i32, i32, pages[:, :1].T), (i32[:0], i32[:0], pages[:0])):
+        with pytest.raises((RuntimeError, ValueError)):
+            K.step_tables(*bad, num_tokens=7, max_blocks=1)
+    with pytest.raises(ValueError, match="must have shape"):
+        K.step_tables(i32, i32, pages, num_tokens=7, max_blocks=1, out=K.StepTables.empty(2, 6, 1, "cuda"))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        K.step_tables(i32, i32, pages, num_tokens=7, max_blocks=1, error_flag=torch.zeros(1, dtype=torch.int32))
+
+    c = rotary_case(4, 2, 1, 64, 32, 2, BF16, 50)
+    d = {k: t.cuda() for k, t in c.items() if torch.is_tensor(t)}
+    q, k, v = views(d["qkv"], c)
+    good = dict(positions=d["positions"], slot_mapping=d["slots"], k_cache=d["kc"], v_cache=d["vc"], omega=d["omega"],
+                axis_of_frequency=d["axis"])
+    K.rotary_write(q, k, v, **good)
+    for bad in (dict(axis_of_frequency=None), dict(positions=d["positions"].int()), dict(slot_mapping=d["slots"][:3]),
+                dict(k_cache=d["kc"][:, :64]), dict(k_cache=d["kc"].to(FP16), v_cache=d["vc"].to(FP16)),
+                dict(omega=d["omega"].double()), dict(q_out=q[:3]), dict(omega=d["omega"][:12], axis_of_frequency=d["axis"][:12])):
+        with pytest.raises((RuntimeError, ValueError)):
+            K.rotary_write(q, k, v, **{**good, **bad})
+    for q1, k1, v1 in ((q[:, :, :32], k, v), (q, k[:3], v[:3]), (q.float(), k, v), (q.transpose(1, 2), k, v)):
+        with pytest.raises((RuntimeError, ValueError)):
+            K.rotary_write(q1, k1, v1, **good)
+
+    a = attention_case([1, 2], [100, 200], 4, 2, 64, BF16)
+    args = [a[x].cuda() for x in ("q", "kc", "vc", "table")] + [ints(a["starts"]), ints(a["lens"])]
+    K.paged_attention(*args, max_query_len=2)
+    for i, bad in ((0, args[0].to(FP16)), (0, args[0].float()), (1, args[1][:, :, :1]), (1, args[1][:, :, :, :32]),
+                   (3, args[3].long()), (3, args[3][:1]), (4, args[4].long()), (4, args[4][:2]), (5, args[5].float())):
+        with pytest.raises((RuntimeError, ValueError)):
+            K.paged_attention(*args[:i], bad, *args[i + 1:], max_query_len=2)
+    for bad in (dict(scale=0.0), dict(window=-1), dict(sinks=-1), dict(max_query_len=-1), dict(out=args[0][:2]),
+                dict(workspace=torch.empty(64, dtype=torch.uint8, device="cuda"))):
+        with pytest.raises((RuntimeError, ValueError)):
+            K.paged_attention(*args, **{"max_query_len": 2, **bad})
+
+
+@pytest.mark.parametrize("longest", [1, 2, 5, 1000])
+def test_the_longest_length_picks_the_kernel_alone(longest):
+    """A bound that is wrong or generous changes which kernel runs, and nothing past rounding."""
+    c = attention_case([1, 5, 0, 40], [300, 900, 7, 40], 10, 2, 128, BF16)
+    check_attention(c, attend(c, max_query_len=longest))
+
+
+def test_calls_on_two_streams_at_once():
+    c = attention_case([1, 70, 2], [3000, 1200, 64], 10, 2, 128, BF16)
+    d = [c[x].cuda() for x in ("q", "kc", "vc", "table")] + [ints(c["starts"]), ints(c["lens"])]
+    want = K.paged_attention(*d, max_query_len=70)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(K.paged_attention(*d, max_query_len=70))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+
+
+def test_a_step_in_one_graph_follows_new_lengths():
+    """Tables, rotary write and attention captured together, padded to a fixed number of tokens."""
+    g = torch.Generator().manual_seed(9)
+    heads, kvh, dim, cap = 8, 2, 64, 8
+    pages = torch.randperm(24, generator=g).view(3, 8)
+    computed, scheduled = ints([100, 500, 3]), ints([1, 1, 1])
+    x = torch.randn(cap, (heads + 2 * kvh) * dim, generator=g).to(BF16).cuda()
+    caches = [torch.randn(24, 128, kvh, dim, generator=g).to(BF16).cuda() for _ in range(2)]
+    omega = (1e6 ** (-torch.arange(dim // 2) / (dim // 2))).cuda()
+    page_table = pages.int().cuda()
+    q, k, v = (y.unflatten(1, (-1, dim)) for y in x.split([heads * dim, kvh * dim, kvh * dim], 1))
+
+    def step():
+        t = K.step_tables(computed, scheduled, page_table, num_tokens=cap, max_blocks=8)
+        turned = K.rotary_write(q, k, v, t.positions, t.slot_mapping, *caches, omega=omega)
+        return (t, turned, *K.paged_attention(turned, *caches, t.block_table, t.query_start_loc, t.seq_lens,
+                                              max_query_len=cap, return_lse=True))
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        t, turned, out, lse = step()
+    for lens, new in (([100, 500, 3], [1, 1, 1]), ([101, 0, 900], [2, 5, 1]), ([7, 700, 0], [0, 0, 3])):
+        computed.copy_(ints(lens))
+        scheduled.copy_(ints(new))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = R.step_tables(lens, new, [0, 0, 0], pages.tolist(), 1, cap, 8)
+        check_tables(t, want)
+        n = sum(new)
+        c = {"q": turned[:n].cpu(), "kc": caches[0].cpu(), "vc": caches[1].cpu(), "table": torch.tensor(want[5]),
+             "starts": want[0], "lens": want[1]}
+        check_attention(c, (out[:n], lse[:n]))

@@ -19,6 +19,9 @@ that sits on the compression hot path and runs every step:
   981-1010): the per-request offset rows, copied to the device when they change.
 * ``physical_positions_for_slot_mapping`` and ``apply_physical_attention_lengths``
   (provider.py:687-728): the per-decode-step offsets, through ``kvc_decode_offsets``.
+* ``step_tables`` (no reference counterpart: the step's tables are vLLM's there):
+  block tables, slot map, positions and physical lengths of the batch in one
+  launch, for hosts that run ``rotary_write`` and ``paged_attention``.
 
 The runner is duck-typed like the reference's tests do it (``device``,
 ``requests``, ``input_batch``, ``req_indices``, ``seq_lens``,
@@ -36,6 +39,7 @@ from typing import Any
 
 import torch
 
+from ._native import DEV_BLOCK_RANGE, DEV_TOKEN_RANGE
 from .config import KERNEL_BLOCK_SIZE
 from .methods.base import CompressionRequest, CompressionResult, MethodRuntimeSpec
 from .methods.triattention import kernels as K
@@ -359,17 +363,34 @@ class BatchedCompressionProvider:
         cpu[:num_reqs].sub_(self._request_offsets_cpu[:num_reqs].to(cpu.dtype))
         self._physical_lengths_applied = True
 
+    def step_tables(self, computed: torch.Tensor, scheduled: torch.Tensor, page_table: torch.Tensor, *,
+                    num_tokens: int, max_blocks: int, out: K.StepTables | None = None) -> K.StepTables:
+        """Tables of the batch's step, in the order of its rows, compressed requests at their physical slots.
+
+        ``computed`` and ``scheduled`` are the rows' tokens so far (semantic) and new ones, ``page_table`` their
+        scheduler pages; call it after ``after_update_states``, which brings the offset rows up to date.  The
+        lengths are physical already: ``apply_physical_attention_lengths`` is for the runner's own.
+        """
+        rows = computed.numel()
+        if rows > self._request_offsets_device.numel():
+            raise RuntimeError("batch has more requests than the runner's max_num_reqs")
+        return K.step_tables(computed, scheduled, page_table, num_tokens=num_tokens, max_blocks=max_blocks,
+                             offsets=self._request_offsets_device[:rows],
+                             blocks_per_page=self.cache_blocks_per_scheduler_block, out=out, error_flag=self._error)
+
     @property
     def semantic_seq_lens(self) -> tuple[torch.Tensor | None, torch.Tensor | None]:
         """(device, host) semantic lengths saved by the last ``apply_physical_attention_lengths``."""
         return self._semantic_seq_lens_device, self._semantic_seq_lens_cpu
 
     def check_device_errors(self) -> None:
-        """Raise if a decode-offset launch met a request index outside the offsets table."""
+        """Raise if a decode-offset or step-table launch met something that it could not place."""
         if self._error is None:
             return
         torch.cuda.current_stream(self.device).synchronize()
         bits = int(self._error.item())
         if bits:
             self._error.zero_()
+            if bits & (DEV_BLOCK_RANGE | DEV_TOKEN_RANGE):
+                raise RuntimeError("kvc_step_tables met a token or block outside the step's tables")
             raise RuntimeError("kvc_decode_offsets met a request index outside the offsets table")
