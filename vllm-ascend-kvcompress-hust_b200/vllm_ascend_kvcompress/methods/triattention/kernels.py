@@ -38,6 +38,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
@@ -466,12 +467,16 @@ def _call(device: torch.device, name: str, *args) -> None:
         N.check(status, name)
 
 
-def _same_device(device: torch.device, tensors) -> None:
-    for t in tensors:
+def _device_of(first: torch.Tensor, *others: torch.Tensor | None) -> torch.device:
+    """The CUDA device that all of a call's tensors are on."""
+    device = first.device
+    if device.type != "cuda":
+        require_cuda(first)
+    for t in others:
         if t is not None and t.device != device:
-            if t.device.type != "cuda":
-                raise RuntimeError("the B200 TriAttention kernels require CUDA tensors (no CPU fallback)")
+            require_cuda(t)
             raise RuntimeError("all tensors of a call must be on one device")
+    return device
 
 
 def _error_word(error_flag: torch.Tensor | None) -> int | None:
@@ -491,8 +496,7 @@ def _paged_cache(cache: torch.Tensor, name: str) -> int:
     return stride[0]
 
 
-@dataclass(frozen=True)
-class StepTables:
+class StepTables(NamedTuple):
     """Device tables of one serving step (``step_tables``).
 
     query_start_loc [R + 1], seq_lens [R] (physical), request_indices [N] and
@@ -509,12 +513,11 @@ class StepTables:
 
     @staticmethod
     def empty(num_requests: int, num_tokens: int, max_blocks: int, device) -> "StepTables":
-        small = torch.empty(2 * num_requests + 1 + num_tokens + num_requests * max_blocks, dtype=torch.int32,
-                            device=device)
-        starts, lens, request, blocks = small.split((num_requests + 1, num_requests, num_tokens,
-                                                     num_requests * max_blocks))
-        positions, slots = torch.empty((2, num_tokens), dtype=torch.int64, device=device).unbind()
-        return StepTables(starts, lens, positions, slots, request, blocks.view(num_requests, max_blocks))
+        i32, i64, new = torch.int32, torch.int64, torch.empty
+        return StepTables(new(num_requests + 1, dtype=i32, device=device), new(num_requests, dtype=i32, device=device),
+                          new(num_tokens, dtype=i64, device=device), new(num_tokens, dtype=i64, device=device),
+                          new(num_tokens, dtype=i32, device=device),
+                          new(num_requests, max_blocks, dtype=i32, device=device))
 
 
 _INTS = (torch.int32, torch.int64)
@@ -534,9 +537,7 @@ def step_tables(computed: torch.Tensor, scheduled: torch.Tensor, page_table: tor
     the block table, whose entries past a request's blocks are -1.  ``out``
     takes tables of an earlier call or ``StepTables.empty``.
     """
-    require_cuda(computed, scheduled, page_table, offsets)
-    device = computed.device
-    _same_device(device, (scheduled, page_table, offsets, error_flag))
+    device = _device_of(computed, scheduled, page_table, offsets, error_flag)
     R = computed.numel()
     if scheduled.numel() != R or page_table.ndim != 2 or page_table.shape[0] != R or (
             offsets is not None and offsets.numel() != R):
@@ -553,8 +554,7 @@ def step_tables(computed: torch.Tensor, scheduled: torch.Tensor, page_table: tor
     if out is None:
         out = StepTables.empty(R, num_tokens, max_blocks, device)
     else:
-        _same_device(device, (out.query_start_loc, out.seq_lens, out.positions, out.slot_mapping,
-                              out.request_indices, out.block_table))
+        _device_of(computed, *out)
         for t, dtype, shape, name in (
                 (out.query_start_loc, torch.int32, (R + 1,), "query_start_loc"),
                 (out.seq_lens, torch.int32, (R,), "seq_lens"),
@@ -589,10 +589,8 @@ def rotary_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: t
     as the calibration statistics assume.  Returns the rotated queries
     (``q_out``, which may be ``q``; a new tensor by default).
     """
-    require_cuda(q, k, v, positions, slot_mapping, k_cache, v_cache, omega, axis_of_frequency, q_out)
-    device, dtype = q.device, q.dtype
-    _same_device(device, (k, v, positions, slot_mapping, k_cache, v_cache, omega, axis_of_frequency, q_out,
-                          error_flag))
+    device, dtype = _device_of(q, k, v, positions, slot_mapping, k_cache, v_cache, omega, axis_of_frequency, q_out,
+                               error_flag), q.dtype
     code = _dtype_code(dtype)
     if q.ndim != 3 or k.ndim != 3 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
         raise ValueError("q must be [tokens, heads, dim], k and v [tokens, kv_heads, dim]")
@@ -603,7 +601,7 @@ def rotary_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: t
     if k.dtype != dtype or v.dtype != dtype or k_cache.dtype != dtype or v_cache.dtype != dtype:
         raise RuntimeError("q, k, v and the caches must have one dtype")
     if q_out is None:
-        q_out = torch.empty((n, heads, dim), dtype=dtype, device=device)
+        q_out = torch.empty(n, heads, dim, dtype=dtype, device=device)
     elif q_out.dtype != dtype or q_out.shape != q.shape:
         raise RuntimeError("q_out must have q's dtype and shape")
     qs, ks, vs, os = q.stride(), k.stride(), v.stride(), q_out.stride()
@@ -654,9 +652,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     allocated per call unless given; one given must not serve two calls that
     run at the same time.
     """
-    require_cuda(q, k_cache, v_cache, block_table, query_start_loc, seq_lens, out, workspace)
-    device, dtype = q.device, q.dtype
-    _same_device(device, (k_cache, v_cache, block_table, query_start_loc, seq_lens, out, workspace, error_flag))
+    device, dtype = _device_of(q, k_cache, v_cache, block_table, query_start_loc, seq_lens, out, workspace,
+                               error_flag), q.dtype
     code = _dtype_code(dtype)
     if q.ndim != 3 or k_cache.ndim != 4 or k_cache.shape != v_cache.shape or k_cache.shape[3] != q.shape[2]:
         raise ValueError("q must be [tokens, heads, dim] and the caches [blocks, 128, kv_heads, dim]")
@@ -671,13 +668,13 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if block_table.dtype != torch.int32 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
         raise RuntimeError("block_table must be int32 with unit inner stride")
     if out is None:
-        out = torch.empty((n, heads, dim), dtype=dtype, device=device)
+        out = torch.empty(n, heads, dim, dtype=dtype, device=device)
     elif out.dtype != dtype or out.shape != q.shape:
         raise RuntimeError("out must have q's dtype and shape")
     qs, os = q.stride(), out.stride()
     if qs[2] != 1 or os[2] != 1:
         raise RuntimeError("q and out must have a contiguous last dim")
-    lse = torch.empty((n, heads), dtype=torch.float32, device=device) if return_lse else None
+    lse = torch.empty(n, heads, dtype=torch.float32, device=device) if return_lse else None
     if workspace is None:
         size = N.lib().kvc_paged_attention_workspace_bytes(max_query_len, heads, kvh, dim)
         workspace = torch.empty(size, dtype=torch.uint8, device=device)
