@@ -6,7 +6,7 @@
 // each of the G query heads: two orders of magnitude under the tensor cores'
 // rate.  So the tile is as small as the tensor instruction allows (16 rows:
 // the heads of one KV head, for as many tokens as fit) and everything serves
-// the stream: one persistent CTA per SM whose TMA producer keeps 96 KB and more of
+// the stream: one persistent CTA per SM whose TMA producer keeps 128 to 192 KB of
 // K/V blocks in flight, four consumer warps that split a block's keys, so no
 // warp waits for another inside a tile, and a line of units cut evenly over the
 // SMs, so a batch of unlike lengths ends everywhere at once.
@@ -39,12 +39,14 @@ struct Geom {
   static constexpr int KB = D <= 128 ? 128 : 64;   // keys per unit (rows_keys)
   static constexpr int kTile = KB * D * 2;         // bytes of a K (or V) block
   static constexpr int kStage = 2 * kTile;
-  static constexpr int kMerge = kConsumers * kRows * D * 4;
-  static constexpr int kFit = (220 * 1024 - kMerge) / kStage;
+  static constexpr int kPitch = D + 8;             // of a row in the merge buffers: 8 rows on different banks
+  static constexpr int kMerge = kConsumers * kRows * kPitch * 4;
+  static constexpr int kFit = (226 * 1024 - kMerge) / kStage;
   static constexpr int kStages = kFit > 6 ? 6 : kFit;
+  static constexpr int kTail = kConsumers * kRows * 8 + kStages * (2 * 8 + 4);  // (m, l) of the warps, barriers, keys
   static constexpr int kKeys = KB / kConsumers;    // keys per warp and unit
-  static constexpr int kSmem = 1024 + kStages * kStage + kMerge;
-  static_assert(kStages >= 2 && kSmem <= 226 * 1024, "shared memory");
+  static constexpr int kSmem = kStages * kStage + kMerge + kTail;
+  static_assert(kStages >= 2 && kSmem <= 227 * 1024, "shared memory");
   static_assert(kStages * kStage >= (kMaxAttendRequests + 41) * 4, "the prefix sums lie in the stages");
 };
 
@@ -112,14 +114,20 @@ __global__ void __launch_bounds__(kThreads, 1) attend_rows_kernel(const __grid_c
   constexpr int KB = G_::KB, S = G_::kStages, NK = G_::kKeys;
   pdl_wait();
   pdl_trigger();
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* merge_o = reinterpret_cast<float*>(base + S * G_::kStage);  // [warp][row][D]
-  __shared__ float2 merge_ml[kConsumers][kRows];
-  __shared__ __align__(8) uint64_t bars[2 * S];
-  __shared__ int stage_key[S];  // first key of the stage's block, or -1 when there is none to read
+  extern __shared__ __align__(1024) uint8_t base[];
+  float* merge_o = reinterpret_cast<float*>(base + S * G_::kStage);  // [warp][row][kPitch]
+  auto merge_ml = reinterpret_cast<float2(*)[kRows]>(base + S * G_::kStage + G_::kMerge);  // [warp][row]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(merge_ml + kConsumers);
+  volatile int* stage_key = reinterpret_cast<int*>(bars + 2 * S);  // first key of the stage's block, or -1: none to read
   const uint32_t stage0 = smem_u32(base), full0 = smem_u32(bars), empty0 = full0 + 8 * S;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if ((stage0 & 1023u) != 0) {  // the swizzle goes by the address
+    if (tid == 0) {
+      raise_flag(a.error_flag, KVC_DEV_TIMEOUT);
+      a.record[blockIdx.x] = make_int4(0, 0, 0, 0);
+    }
+    return;
+  }
   if (tid == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(full0 + 8 * s, 1);
@@ -326,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_rows_kernel(const __grid_c
       l[j] += __shfl_xor_sync(0xffffffffu, l[j], 1);
       l[j] += __shfl_xor_sync(0xffffffffu, l[j], 2);
       if ((lane & 3) == 0) merge_ml[warp][lane / 4 + 8 * j] = make_float2(m[j], l[j]);
-      float* dst = merge_o + (warp * kRows + lane / 4 + 8 * j) * D + 2 * (lane & 3);
+      float* dst = merge_o + (warp * kRows + lane / 4 + 8 * j) * G_::kPitch + 2 * (lane & 3);
 #pragma unroll
       for (int i = 0; i < D / 8; ++i) *reinterpret_cast<float2*>(dst + 8 * i) = make_float2(o[i][2 * j], o[i][2 * j + 1]);
     }
@@ -345,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_rows_kernel(const __grid_c
         const float2 ml = merge_ml[w][row];
         // an empty part has o = l = 0, or, with values that are not finite, what it has to add
         const float f = ml.x == -INFINITY ? 1.f : exp2_approx((ml.x - mx) * a.scale_log2);
-        const float4 v = *reinterpret_cast<const float4*>(merge_o + (w * kRows + row) * D + d);
+        const float4 v = *reinterpret_cast<const float4*>(merge_o + (w * kRows + row) * G_::kPitch + d);
         sum += f * ml.y;
         acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
       }
@@ -367,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_rows_kernel(const __grid_c
     if (c.left == 0 && tid == 0) {
       int4 rec = make_int4(0, t.row0, t.ntok, c.h);
       if (starts && !ends) {  // later CTAs hold the rest of this tile
-        const int64_t u1 = ((int64_t)blockIdx.x + 1) * line.total / line.used;
+        const int64_t u1 = attend_div(((int64_t)blockIdx.x + 1) * line.total, line.used);
         rec.x = (int)(attend_owner(line, u1 - 1 + (t.units - n)) - blockIdx.x);
       }
       a.record[blockIdx.x] = rec;
@@ -590,7 +598,6 @@ extern "C" int kvc_paged_attention(const void* q, int64_t q_token_stride, int64_
   a.window = window, a.sinks = window > 0 ? sinks : 0;
   a.sub = 128 / a.G;
   a.tok = wide ? a.rows / 128 * a.sub : kRows / a.G;
-  a.min_units = 1;
   a.scale = scale;
   a.scale_log2 = scale * 1.44269504088896340736f;
   const int keys = wide ? attend_umma_slot_keys(head_dim) : rows_keys(head_dim);

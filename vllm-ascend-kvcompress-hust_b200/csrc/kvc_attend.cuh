@@ -52,7 +52,6 @@ struct AttendArgs {
   int sub;   // tokens per 128-row half of a tile (tcgen05 kernel)
   int rows;  // rows of a partial
   int ctas;  // CTAs that share the line of units
-  int min_units;
   float scale, scale_log2;
 };
 
@@ -100,15 +99,19 @@ struct AttendCursor {
   int64_t left;  // units of this CTA from here on
 };
 
-// where the line stands
+// the line, and how it is shared: CTA c has the units [c * total / used, (c + 1) * total / used)
 struct AttendLine {
   int64_t total;  // units of all KV heads
   int64_t used;   // CTAs that have work
 };
 
+// a / b, a < 2^53: a quotient that is no whole number lies 1 / b under the next one, more than the division's
+// rounding (a few dozen instructions, against a few hundred for 64-bit integers)
+__device__ __forceinline__ int64_t attend_div(int64_t a, int64_t b) { return (int64_t)__ddiv_rd((double)a, (double)b); }
+
 // CTA that owns unit x when `used` CTAs share `total` units as [c * total / used, (c + 1) * total / used)
 __device__ __forceinline__ int64_t attend_owner(const AttendLine& l, int64_t x) {
-  return ((x + 1) * l.used - 1) / l.total;
+  return attend_div((x + 1) * l.used - 1, l.total);
 }
 
 // All threads: this CTA's piece of the line.  `sh`: R + 1 + 40 ints of shared memory, free again on return.
@@ -172,12 +175,12 @@ __device__ AttendCursor attend_locate(const AttendArgs& a, int32_t* sh, AttendLi
   }
   AttendCursor c{0, 0, 0, 0, 0};
   line->total = sum * a.Hkv;
-  line->used = sum == 0 ? 0 : max((int64_t)1, min((int64_t)a.ctas, line->total / a.min_units));
+  line->used = min((int64_t)a.ctas, line->total);
   int32_t* found = sh + 34;
   if ((int64_t)blockIdx.x < line->used) {  // the same for the whole CTA
-    const int64_t u0 = (int64_t)blockIdx.x * line->total / line->used;
-    const int64_t u1 = ((int64_t)blockIdx.x + 1) * line->total / line->used;
-    const int64_t want = u0 % sum;
+    const int64_t u0 = attend_div((int64_t)blockIdx.x * line->total, line->used);
+    const int64_t u1 = attend_div(((int64_t)blockIdx.x + 1) * line->total, line->used);
+    const int64_t h = attend_div(u0, sum), want = u0 - h * sum;
     int64_t base = 0;
     for (int t0 = 0; t0 < tiles; t0 += NT) {
       if (tiles > NT) {
@@ -198,7 +201,7 @@ __device__ AttendCursor attend_locate(const AttendArgs& a, int32_t* sh, AttendLi
       if (base > want) break;
     }
     __syncthreads();
-    c = AttendCursor{(int)(u0 / sum), found[0], found[1], found[2], u1 - u0};
+    c = AttendCursor{(int)h, found[0], found[1], found[2], u1 - u0};
   }
   __syncthreads();
   return c;

@@ -668,7 +668,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
       if (c.left == 0 && tid == 0) {
         int4 rec = make_int4(0, t.row0, t.ntok, c.h);
         if (starts && !ends) {  // later CTAs hold the rest of this tile
-          const int64_t u1 = ((int64_t)blockIdx.x + 1) * line.total / line.used;
+          const int64_t u1 = attend_div(((int64_t)blockIdx.x + 1) * line.total, line.used);
           rec.x = (int)(attend_owner(line, u1 - 1 + (t.units - n)) - blockIdx.x);
         }
         a.record[blockIdx.x] = rec;
