@@ -475,6 +475,13 @@ def test_the_longest_length_picks_the_kernel_alone(longest):
     check_attention(c, attend(c, max_query_len=longest))
 
 
+@pytest.mark.parametrize("new", [[1, 1], [1, 90]])
+@pytest.mark.parametrize("window,sinks", [(2 ** 31 - 1, 2 ** 31 - 1), (30, 2 ** 31 - 1), (2 ** 31 - 1, 0)])
+def test_windows_and_first_tokens_past_any_cache(new, window, sinks):
+    c = attention_case(new, [200, 300], 4, 2, 128, BF16)
+    check_attention(c, attend(c, window=window, sinks=sinks), window, sinks)
+
+
 def test_calls_on_two_streams_at_once():
     c = attention_case([1, 70, 2], [3000, 1200, 64], 10, 2, 128, BF16)
     d = [c[x].cuda() for x in ("q", "kc", "vc", "table")] + [ints(c["starts"]), ints(c["lens"])]

@@ -42,7 +42,7 @@ def test_rotary_write_refusals():
         assert rotary(**{name: None}) == -14, name
     assert rotary(axes=3) == -14  # several axes need the axis of each frequency
     for bad in ({"dtype": 2}, {"n": -1}, {"heads": 0}, {"kvh": 0}, {"blocks": 0}, {"rot": 0}, {"rot": 144},
-                {"axes": 0}, {"axes": 9}, {"kb": 128 * 256 - 8}, {"ps": -1}):
+                {"axes": 0}, {"axes": 9}, {"kb": 128 * 256 - 8}, {"ps": -1}, {"o0": 0}, {"o1": 0}):
         assert rotary(**bad) == -22, bad
     for bad in ({"rot": 24}, {"dim": 132, "rot": 128}, {"dim": 512, "rot": 272, "kb": 1 << 20, "vb": 1 << 20}):
         assert rotary(**bad) == -95, bad

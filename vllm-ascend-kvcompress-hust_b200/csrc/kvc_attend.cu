@@ -595,7 +595,8 @@ extern "C" int kvc_paged_attention(const void* q, int64_t q_token_stride, int64_
   a.table_stride = table_stride, a.table_width = table_width, a.num_blocks = (int)num_blocks;
   a.num_tokens = num_tokens;
   a.R = num_requests, a.Hq = heads, a.Hkv = kv_heads, a.G = heads / kv_heads, a.D = head_dim;
-  a.window = window, a.sinks = window > 0 ? sinks : 0;
+  // past any cache: 2^30 is as good as more, and positions plus or minus it stay inside an int
+  a.window = std::min(window, 1 << 30), a.sinks = window > 0 ? std::min(sinks, 1 << 30) : 0;
   a.sub = 128 / a.G;
   a.tok = wide ? a.rows / 128 * a.sub : kRows / a.G;
   a.scale = scale;

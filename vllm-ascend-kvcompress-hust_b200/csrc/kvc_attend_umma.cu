@@ -2,30 +2,39 @@
 // (tcgen05, sm_100a).  kvc_attend.cuh has the mathematics and how work is
 // shared out.
 //
-// Bound: the tensor cores (4 D flops per row and visible key) and, next to
-// them, the SM's exponential unit: 128 keys x 128 rows are 16,384 exponentials
-// at 16 a cycle, 1024 cycles, against 8 D cycles of tensor work (1024 at
-// head_dim 128, half of that at 64).
+// Bound: the tensor cores (4 D flops per row and visible key), the SM's
+// exponential unit beside them (128 keys x 128 rows are 16,384 exponentials at
+// 16 a cycle, 1024 cycles, against 8 D cycles of tensor work) and, in a run of
+// such calls, the 1000 W cap.  2048 new tokens over 16,384 at 40 / 8 heads of 128:
+// 0.82 ms, 890 TFLOP/s, 0.54 of the measured burst rate at 1.45 to 1.65 GHz; the
+// same kernel takes 0.60 to 0.65 ms at 1.9 GHz, and changes that saved a tenth
+// of its cycles (an eighth of the exponentials as polynomials on the FMA pipes)
+// left its time as it was.
 //
 // Roles of a CTA (one per SM: it holds all 512 TMEM columns):
 //  * producer lane: queries of each tile and K/V blocks of 16 or 32 KB into a
 //    ring of shared-memory slots, by TMA with the 128-byte swizzle;
-//  * MMA lane: S = Q K^T with both operands in shared memory, O += P V with P
-//    from tensor memory (it overwrites the S it came from) and V read from the
-//    very tile that TMA wrote, as an N-major operand: nothing is transposed;
+//  * two MMA lanes: S = Q K^T with both operands in shared memory, O += P V with
+//    P from tensor memory and V read from the very tile that TMA wrote, as an
+//    N-major operand: nothing is transposed;
 //  * two softmax warpgroups: a thread owns one row, so maximum and sum need no
 //    exchange; S row from TMEM, masked, 2^(c s - c m), rounded to the cache's
 //    type (the instruction wants A and B alike; off by half a step of the
 //    weight at most, as the output's own rounding) and stored back as P.
-// head_dim 64 and 128: a tile has two halves of 128 rows, one per warpgroup,
-// that share every K/V block, and the MMA lane alternates between them, so one
-// half's products run under the other's exponentials.  head_dim 256: O alone
-// takes 256 columns, so a tile has 128 rows, S is double-buffered and each
-// warpgroup takes 64 of a block's 128 keys (row maxima by shared memory).
+// head_dim 64 and 128: a tile has two halves of 128 rows, one per warpgroup and
+// MMA lane, that share every K/V block.  S comes in parts of 64 keys with two
+// buffers to a half (P goes over the S it came from): the next part's S is
+// computed under this one's exponentials.  S of 128 keys at a time left no TMEM
+// for that, and each product then waited for the exponentials before it (955 us
+// for the above).  head_dim 256: O alone takes 256 columns, so a tile has 128
+// rows, P lies beside S, and each warpgroup takes 64 of a block's 128 keys (row
+// maxima by shared memory).
 //
-// The running maximum is raised only when a block's exceeds it by 2^8: weights
-// up to 256 lose nothing in fp32, bf16 or fp16, and the output in TMEM is
-// rescaled in the first blocks of a row alone.
+// The maximum that the weights are taken with is raised only when it has to be:
+// when a part's own exceeds it by 2^8, which at head_dim 64 and 128 is looked at
+// only when the sum of 64 weights passes 2^15, so that most parts need no pass
+// over the scores for their maximum.  Weights above 1 lose nothing in fp32, bf16
+// or fp16, and the output in TMEM is rescaled in the first parts of a row alone.
 //
 // Every wait is bounded (KVC_DEV_TIMEOUT); a softmax warp whose wait ran out
 // goes on without waiting, so every named barrier is met, the other roles
@@ -460,156 +469,156 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
           const bool whole = attend_whole(a, t.pos0, t.last(), k0, KB);  // for the tile
 #pragma unroll 1
           for (int part = NT == 1 ? wg : 0; part < 2; part += NT == 1 ? 2 : 1) {  // 64 keys of the block
-          wait(sfull + 16 * half + (NT == 2 ? 8 * part : 0), g & 1);
-          tc_fence_after();
-          const bool skip = (meta[ga % kMeta] & kSkip) != 0;
-          const uint32_t scol = lane_base + G_::s_col(half, part), pcol = lane_base + G_::p_col(half, part, g);
-          uint32_t w[64];  // the row's scores
-          float* s = reinterpret_cast<float*>(w);
-          tmem_ld32_async(scol, w);
-          tmem_ld32_async(scol + 32, w + 32);
-          if (!skip && !whole && (NT == 1 || part == 0)) {
-            // A masked key weighs nothing whatever its value row holds, but 0 * inf
-            // is not 0 in the product: infinite and NaN values leave the block
-            // here and reach the rows that do see them by addition at the end.
-            const uint32_t vs = HV * G_::v_at(ga, units);
-            if (NT == 1 && g > 0) wait_o(g, 0);  // its V has been in the slots before this one's
+            wait(sfull + 16 * half + (NT == 2 ? 8 * part : 0), g & 1);
+            tc_fence_after();
+            const bool skip = (meta[ga % kMeta] & kSkip) != 0;
+            const uint32_t scol = lane_base + G_::s_col(half, part), pcol = lane_base + G_::p_col(half, part, g);
+            uint32_t w[64];  // the row's scores
+            float* s = reinterpret_cast<float*>(w);
+            tmem_ld32_async(scol, w);
+            tmem_ld32_async(scol + 32, w + 32);
+            if (!skip && !whole && (NT == 1 || part == 0)) {
+              // A masked key weighs nothing whatever its value row holds, but 0 * inf
+              // is not 0 in the product: infinite and NaN values leave the block
+              // here and reach the rows that do see them by addition at the end.
+              const uint32_t vs = HV * G_::v_at(ga, units);
+              if (NT == 1 && g > 0) wait_o(g, 0);  // its V has been in the slots before this one's
 #pragma unroll
-            for (int hv = 0; hv < HV; ++hv) wait(full0 + 8 * ((vs + hv) % S), ((vs + hv) / S) & 1);
-            bool odd = false;
-            constexpr int kVec = KB * D / 8;
-            auto vaddr = [&](int i) { return ring0 + ((vs + i / (SK * D / 8)) % S) * G_::kSlot + (i % (SK * D / 8)) * 16; };
-            // Each warpgroup looks for itself (with one half they share the block), and nothing is cleared
-            // before both have looked, so both find the same.
-            constexpr int kLook = NT == 1 ? 256 : 128;
-            for (int i = tid % kLook; i < kVec; i += kLook) {
-              uint32_t w[4];
-              lds128(vaddr(i), w);
-              odd |= odd_pair<FP16>(w[0]) | odd_pair<FP16>(w[1]) | odd_pair<FP16>(w[2]) | odd_pair<FP16>(w[3]);
-            }
-            const int team = NT == 1 || halves == 2 ? 256 : 128;
-            if (named_or(2 + (NT == 1 ? 0 : wg), kLook, odd)) {
-              const int d0 = NT == 1 ? wg * OC : 0;
-              if (live && !poison) {
-                for (int d = 0; d < OC; ++d) mine[d] = 0.f;
-                poison = true;
-              }
-              for (int key = 0; key < KB; ++key) {
-                if (!live || !attend_sees(a, pos, k0 + key)) continue;
-                const int row = key % SK;
-                const uint32_t slot = ring0 + ((vs + key / SK) % S) * G_::kSlot;
-                for (int d = d0; d < d0 + OC; d += 2) {
-                  uint32_t w;
-                  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w)
-                               : "r"(slot + (d / kSpan) * G_::kBox + row * 128 + ((((d % kSpan) / 8) ^ (row & 7)) << 4) +
-                                     (d % 8) * 2)
-                               : "memory");
-                  if (!odd_pair<FP16>(w)) continue;
-                  const float2 v = unpack2(w, E{});
-                  if (!isfinite(v.x)) mine[d - d0] += v.x;
-                  if (!isfinite(v.y)) mine[d - d0 + 1] += v.y;
-                }
-              }
-              named_sync(team);  // read by all before it is cleared
-              for (int i = team == 256 ? tid : r; i < kVec; i += team) {
-                const uint32_t ad = vaddr(i);
+              for (int hv = 0; hv < HV; ++hv) wait(full0 + 8 * ((vs + hv) % S), ((vs + hv) / S) & 1);
+              bool odd = false;
+              constexpr int kVec = KB * D / 8;
+              auto vaddr = [&](int i) { return ring0 + ((vs + i / (SK * D / 8)) % S) * G_::kSlot + (i % (SK * D / 8)) * 16; };
+              // Each warpgroup looks for itself (with one half they share the block), and nothing is cleared
+              // before both have looked, so both find the same.
+              constexpr int kLook = NT == 1 ? 256 : 128;
+              for (int i = tid % kLook; i < kVec; i += kLook) {
                 uint32_t w[4];
-                lds128(ad, w);
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  if (odd_pair<FP16>(w[j])) {
-                    const float2 v = unpack2(w[j], E{});
-                    w[j] = (isfinite(v.x) ? w[j] & 0xffffu : 0u) | (isfinite(v.y) ? w[j] & 0xffff0000u : 0u);
-                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(ad + 4 * j), "r"(w[j]) : "memory");
+                lds128(vaddr(i), w);
+                odd |= odd_pair<FP16>(w[0]) | odd_pair<FP16>(w[1]) | odd_pair<FP16>(w[2]) | odd_pair<FP16>(w[3]);
+              }
+              const int team = NT == 1 || halves == 2 ? 256 : 128;
+              if (named_or(2 + (NT == 1 ? 0 : wg), kLook, odd)) {
+                const int d0 = NT == 1 ? wg * OC : 0;
+                if (live && !poison) {
+                  for (int d = 0; d < OC; ++d) mine[d] = 0.f;
+                  poison = true;
+                }
+                for (int key = 0; key < KB; ++key) {
+                  if (!live || !attend_sees(a, pos, k0 + key)) continue;
+                  const int row = key % SK;
+                  const uint32_t slot = ring0 + ((vs + key / SK) % S) * G_::kSlot;
+                  for (int d = d0; d < d0 + OC; d += 2) {
+                    uint32_t w;
+                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w)
+                                 : "r"(slot + (d / kSpan) * G_::kBox + row * 128 + ((((d % kSpan) / 8) ^ (row & 7)) << 4) +
+                                       (d % 8) * 2)
+                                 : "memory");
+                    if (!odd_pair<FP16>(w)) continue;
+                    const float2 v = unpack2(w, E{});
+                    if (!isfinite(v.x)) mine[d - d0] += v.x;
+                    if (!isfinite(v.y)) mine[d - d0 + 1] += v.y;
                   }
+                }
+                named_sync(team);  // read by all before it is cleared
+                for (int i = team == 256 ? tid : r; i < kVec; i += team) {
+                  const uint32_t ad = vaddr(i);
+                  uint32_t w[4];
+                  lds128(ad, w);
+#pragma unroll
+                  for (int j = 0; j < 4; ++j)
+                    if (odd_pair<FP16>(w[j])) {
+                      const float2 v = unpack2(w[j], E{});
+                      w[j] = (isfinite(v.x) ? w[j] & 0xffffu : 0u) | (isfinite(v.y) ? w[j] & 0xffff0000u : 0u);
+                      asm volatile("st.shared.b32 [%0], %1;" ::"r"(ad + 4 * j), "r"(w[j]) : "memory");
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                named_sync(team);
               }
-              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-              named_sync(team);
             }
-          }
-          tmem_ld_wait();
-          tmem_ready32(w);
-          tmem_ready32(w + 32);
-          if (NT == 1) {
-            arrive(sread);
-            if (g > 1) wait_o(g - 1, 0);  // the unit before the last has left P's place
-          }
-          if (!skip) {
-            // weights of the 64 keys, rounded into p; returns the sum of the unrounded ones
-            uint32_t p[32];
-            auto weigh = [&]() {
-              const float ms = m == -INFINITY ? 0.f : m * a.scale_log2;
-              const float2 c2 = make_float2(a.scale_log2, a.scale_log2), n2 = make_float2(-ms, -ms);
-              float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            tmem_ld_wait();
+            tmem_ready32(w);
+            tmem_ready32(w + 32);
+            if (NT == 1) {
+              arrive(sread);
+              if (g > 1) wait_o(g - 1, 0);  // the unit before the last has left P's place
+            }
+            if (!skip) {
+              // weights of the 64 keys, rounded into p; returns the sum of the unrounded ones
+              uint32_t p[32];
+              auto weigh = [&]() {
+                const float ms = m == -INFINITY ? 0.f : m * a.scale_log2;
+                const float2 c2 = make_float2(a.scale_log2, a.scale_log2), n2 = make_float2(-ms, -ms);
+                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                const float2 x = __ffma2_rn(make_float2(s[2 * j], s[2 * j + 1]), c2, n2);
-                const float2 e = make_float2(exp2_approx(x.x), exp2_approx(x.y));
-                sum[j & 1] = __fadd2_rn(sum[j & 1], e);
-                p[j] = pack<FP16>(e.x, e.y);
-              }
-              sum[0] = __fadd2_rn(sum[0], sum[1]);
-              return sum[0].x + sum[0].y;
-            };
-            auto largest = [&]() {
-              float top[4] = {s[0], s[1], s[2], s[3]};
+                for (int j = 0; j < 32; ++j) {
+                  const float2 x = __ffma2_rn(make_float2(s[2 * j], s[2 * j + 1]), c2, n2);
+                  const float2 e = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+                  sum[j & 1] = __fadd2_rn(sum[j & 1], e);
+                  p[j] = pack<FP16>(e.x, e.y);
+                }
+                sum[0] = __fadd2_rn(sum[0], sum[1]);
+                return sum[0].x + sum[0].y;
+              };
+              auto largest = [&]() {
+                float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-              for (int j = 4; j < 60; j += 8)
+                for (int j = 4; j < 60; j += 8)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) top[k] = max3(top[k], s[j + k], s[j + 4 + k]);
+                  for (int k = 0; k < 4; ++k) top[k] = max3(top[k], s[j + k], s[j + 4 + k]);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) top[k] = fmaxf(top[k], s[60 + k]);
-              return max3(fmaxf(top[0], top[1]), top[2], top[3]);
-            };
-            // a new maximum: the row's sum and its output so far times f
-            auto rescale = [&](float f) {
-              l *= f;
-              wait_o(g, NT == 1 ? 0 : part);
+                for (int k = 0; k < 4; ++k) top[k] = fmaxf(top[k], s[60 + k]);
+                return max3(fmaxf(top[0], top[1]), top[2], top[3]);
+              };
+              // a new maximum: the row's sum and its output so far times f
+              auto rescale = [&](float f) {
+                l *= f;
+                wait_o(g, NT == 1 ? 0 : part);
 #pragma unroll 1
-              for (int i = 0; i < OC; i += 32) {
-                uint32_t o[32];
-                tmem_ld32(ocol + i, o);
+                for (int i = 0; i < OC; i += 32) {
+                  uint32_t o[32];
+                  tmem_ld32(ocol + i, o);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-                tmem_st32(ocol + i, o);
+                  for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                  tmem_st32(ocol + i, o);
+                }
+              };
+              float sum = 0.f;
+              // The weights are taken with the maximum as it stands, and only a sum that is too large (or a row's
+              // first keys) asks for the scores' own: no pass for the maximum in most blocks.
+              bool fine = false;
+              const bool seen = whole || attend_whole(a, pos_first, pos_last, k0 + 64 * part, 64);  // by this half's rows
+              if (NT == 2 && seen && ready) {
+                sum = weigh();
+                fine = __all_sync(0xffffffffu, !live || sum <= kMost);
               }
-            };
-            float sum = 0.f;
-            // The weights are taken with the maximum as it stands, and only a sum that is too large (or a row's
-            // first keys) asks for the scores' own: no pass for the maximum in most blocks.
-            bool fine = false;
-            const bool seen = whole || attend_whole(a, pos_first, pos_last, k0 + 64 * part, 64);  // by this half's rows
-            if (NT == 2 && seen && ready) {
-              sum = weigh();
-              fine = __all_sync(0xffffffffu, !live || sum <= kMost);
-            }
-            if (__builtin_expect(!fine, 0)) {
-              if (!seen) {
-                const int c0 = k0 + 64 * part;  // attend_sees, relative to the row's columns
-                const int hi = pos - c0, lo = a.window > 0 ? hi - a.window : -1, first = a.sinks - c0;
+              if (__builtin_expect(!fine, 0)) {
+                if (!seen) {
+                  const int c0 = k0 + 64 * part;  // attend_sees, relative to the row's columns
+                  const int hi = pos - c0, lo = a.window > 0 ? hi - a.window : -1, first = a.sinks - c0;
 #pragma unroll
-                for (int j = 0; j < 64; ++j) s[j] = j <= hi && (j > lo || j < first) ? s[j] : -INFINITY;
+                  for (int j = 0; j < 64; ++j) s[j] = j <= hi && (j > lo || j < first) ? s[j] : -INFINITY;
+                }
+                float mx = largest();
+                if constexpr (NT == 1) {
+                  xch[((g & 1) * 2 + wg) * 128 + r] = mx;
+                  named_sync(256);
+                  mx = fmaxf(mx, xch[((g & 1) * 2 + (wg ^ 1)) * 128 + r]);
+                }
+                const bool raise = !(mx <= m) && (m == -INFINITY || !((mx - m) * a.scale_log2 <= kSlack));  // or NaN
+                const float f = raise && m > -INFINITY ? exp2_approx((m - mx) * a.scale_log2) : 1.f;
+                if (raise) m = mx;
+                if (__any_sync(0xffffffffu, f != 1.f)) rescale(f);
+                sum = weigh();
+                if (live && !(sum <= kMost)) sum = NAN;  // a score is infinite or NaN
+                ready = __all_sync(0xffffffffu, !live || m > -INFINITY);
               }
-              float mx = largest();
-              if constexpr (NT == 1) {
-                xch[((g & 1) * 2 + wg) * 128 + r] = mx;
-                named_sync(256);
-                mx = fmaxf(mx, xch[((g & 1) * 2 + (wg ^ 1)) * 128 + r]);
-              }
-              const bool raise = !(mx <= m) && (m == -INFINITY || !((mx - m) * a.scale_log2 <= kSlack));  // or NaN
-              const float f = raise && m > -INFINITY ? exp2_approx((m - mx) * a.scale_log2) : 1.f;
-              if (raise) m = mx;
-              if (__any_sync(0xffffffffu, f != 1.f)) rescale(f);
-              sum = weigh();
-              if (live && !(sum <= kMost)) sum = NAN;  // a score is infinite or NaN
-              ready = __all_sync(0xffffffffu, !live || m > -INFINITY);
+              l += sum;
+              any = true;
+              tmem_st32(pcol, p);
+              tc_wait_st();
             }
-            l += sum;
-            any = true;
-            tmem_st32(pcol, p);
-            tc_wait_st();
-          }
-          arrive(pfull + 16 * half + 8 * part);
+            arrive(pfull + 16 * half + 8 * part);
           }
         }
         // ---- the piece's output ----

@@ -185,6 +185,7 @@ extern "C" int kvc_rotary_write(const void* q, int64_t q_token_stride, int64_t q
   if (num_tokens == 0) return KVC_OK;
   KVC_CHECK_ARG(q && k && v && positions && omega && slot_mapping && q_out && k_cache && v_cache, KVC_ENULL);
   KVC_CHECK_ARG(axes == 1 || axis_of_frequency, KVC_ENULL);
+  KVC_CHECK_ARG((num_tokens == 1 || out_token_stride > 0) && (heads == 1 || out_head_stride > 0), KVC_EINVAL);
   const int64_t row = (int64_t)kvc::kBlock * kv_heads * head_dim;
   KVC_CHECK_ARG(k_block_stride >= row && v_block_stride >= row, KVC_EINVAL);
   const int64_t strides[] = {q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride,
