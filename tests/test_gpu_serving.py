@@ -370,6 +370,36 @@ def test_results_do_not_depend_on_timing():
         assert torch.equal(K.paged_attention(*d, max_query_len=300), first)
 
 
+@pytest.mark.parametrize("new", [[1, 1], [60, 1]])
+def test_offsets_past_32_bits(new):
+    """Blocks past 4 GB of a cache that interleaves K and V, written by the rotary write and read by attention."""
+    kvh, dim, heads, blocks, n = 8, 128, 16, 9000, sum(new)
+    g = torch.Generator().manual_seed(1)
+    both = torch.zeros(blocks, 2, 128 * kvh * dim, dtype=BF16, device="cuda")
+    kc, vc = (both[:, i].unflatten(1, (128, kvh, dim)) for i in (0, 1))
+    lens, ids = [300, 129], [[8999, 3, 8700], [8500, 8998, -1]]
+    used = [8999, 3, 8700, 8500, 8998]
+    for c in (kc, vc):
+        c[used] = torch.randn(len(used), 128, kvh, dim, generator=g).to(BF16).cuda()
+    x = torch.randn(n, heads + 2 * kvh, dim, generator=g).to(BF16)
+    starts = [0, new[0], n]
+    slots = [ids[r][p // 128] * 128 + p % 128 for r in range(2) for p in range(lens[r] - new[r], lens[r])]
+    pos = torch.arange(n)[None]
+    omega = 1e6 ** (-torch.arange(dim // 2) / (dim // 2))
+    q, k, v = x.cuda().split([heads, kvh, kvh], 1)
+    q = K.rotary_write(q, k, v, pos.cuda(), ints(slots, torch.int64), kc, vc, omega=omega.cuda())
+    small = {i: j for j, i in enumerate(used)}
+    hk, hv = kc[used].cpu(), vc[used].cpu()
+    at = [small[s // 128] * 128 + s % 128 for s in slots]
+    want = R.rotate(x[:, heads: heads + kvh], pos, omega, torch.zeros(dim // 2).long())
+    assert (hk.flatten(0, 1)[at].double() - want).abs().le(R.rotate_bound(x[:, heads: heads + kvh], omega, BF16)).all()
+    assert torch.equal(hv.flatten(0, 1)[at], x[:, heads + kvh:])
+    got = K.paged_attention(q, kc, vc, ints(ids), ints(starts), ints(lens), max_query_len=max(new), return_lse=True)
+    c = {"q": q.cpu(), "kc": hk, "vc": hv, "table": torch.tensor([[small.get(i, -1) for i in row] for row in ids]),
+         "starts": starts, "lens": lens}
+    check_attention(c, got)
+
+
 # ---- a step of all three --------------------------------------------------------------------------
 
 
