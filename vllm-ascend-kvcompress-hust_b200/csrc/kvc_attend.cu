@@ -2,9 +2,8 @@
 // (sm_100a).  kvc_attend.cuh has the mathematics and how work is shared out.
 //
 // Bound: HBM.  A decode step reads every K and V row of its requests once (4 D
-// bytes per key and KV head) and does 4 G D flops on it, 1-4 flops a byte for
-// each of the G query heads: two orders of magnitude under the tensor cores'
-// rate.  So the tile is as small as the tensor instruction allows (16 rows:
+// bytes per key and KV head) and does 4 G D flops on it, a flop a byte for each
+// of the G query heads: two orders of magnitude under the tensor cores' rate.  So the tile is as small as the tensor instruction allows (16 rows:
 // the heads of one KV head, for as many tokens as fit) and everything serves
 // the stream: one persistent CTA per SM whose TMA producer keeps 128 to 192 KB of
 // K/V blocks in flight, four consumer warps that split a block's keys, so no
@@ -22,7 +21,7 @@
 // of O += P V (V by transposing ldmatrix), the sums taken from the unrounded
 // exponentials.  P is rounded to the cache's 16 bits because the tensor
 // instruction wants both operands alike; each weight is off by half a step at
-// most (2^-9 relative to it), independent from key to key, which is no more
+// most (2^-8 of it in bf16, 2^-11 in fp16), independent from key to key, which is no more
 // than the output's own rounding.  mma.sync rather than tcgen05: with 5 to 16
 // of 128 rows in use a 128-row instruction computes mostly padding, and the
 // legacy path is far from being the bound.
@@ -38,6 +37,7 @@ constexpr int kRows = 16;
 constexpr int kConsumers = 4;
 constexpr int kThreads = (kConsumers + 1) * 32;
 constexpr int kSpan = 64;  // elements of a 128-byte swizzle span
+constexpr int kExtra = 2;  // units' time that a tile's start and end take (2,600 cycles, a unit 1,450)
 
 template <int D>
 struct Geom {
@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_rows_kernel(const __grid_c
     mbar_init_fence();
   }
   AttendLine line;
-  AttendCursor c = attend_locate<KB, kThreads>(a, reinterpret_cast<int32_t*>(base), &line);  // synchronises
+  AttendCursor c = attend_locate<KB, kThreads, kExtra>(a, reinterpret_cast<int32_t*>(base), &line);  // synchronises
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the stages held the prefix sums
   __syncthreads();
   const int64_t end = c.left;

@@ -12,7 +12,8 @@
 // tokens of a request (row = token * G + head in group), so a KV block is read
 // once for all the heads that share it.  A *unit* is one KB-key block of a
 // tile that some row sees.  The units of all tiles, KV heads outermost, form
-// one line; each CTA takes an equal piece of it, whatever the requests'
+// one line, on which a tile also takes the room of `Extra` units, about what its
+// start and end cost; each CTA has an equal length of it, whatever the requests'
 // lengths.  A tile whose units all fall to one CTA is finished there; the
 // parts of a tile cut by a CTA boundary go to the workspace as (o, m, l) and
 // attend_combine_kernel joins them in unit order, so results do not depend on
@@ -109,13 +110,13 @@ struct AttendLine {
 // rounding (a few dozen instructions, against a few hundred for 64-bit integers)
 __device__ __forceinline__ int64_t attend_div(int64_t a, int64_t b) { return (int64_t)__ddiv_rd((double)a, (double)b); }
 
-// CTA that owns unit x when `used` CTAs share `total` units as [c * total / used, (c + 1) * total / used)
+// CTA that owns place x of the line
 __device__ __forceinline__ int64_t attend_owner(const AttendLine& l, int64_t x) {
   return attend_div((x + 1) * l.used - 1, l.total);
 }
 
 // All threads: this CTA's piece of the line.  `sh`: R + 1 + 40 ints of shared memory, free again on return.
-template <int KB, int NT>
+template <int KB, int NT, int Extra>
 __device__ AttendCursor attend_locate(const AttendArgs& a, int32_t* sh, AttendLine* line) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int32_t* first = sh + 40;  // [R + 1] tiles before each request
@@ -160,48 +161,53 @@ __device__ AttendCursor attend_locate(const AttendArgs& a, int32_t* sh, AttendLi
     r = lo;
     return t - first[lo];
   };
-  // units of one KV head, and -- when one round of threads covers the tiles -- each tile's place
+  // length of one KV head, and -- when one round of threads covers the tiles -- each tile's place
   int64_t sum = 0;
   int mine = 0, before = 0, my_r = 0, my_i = 0;
-  for (int t0 = 0; t0 < tiles; t0 += NT) {
-    const int t = t0 + tid;
+  auto measure = [&](int t) {
     mine = 0;
     if (t < tiles) {
       my_i = tile_of(t, my_r);
-      mine = attend_tile<KB>(a, my_r, my_i).units;
+      mine = Extra + attend_tile<KB>(a, my_r, my_i).units;
     }
     before = scan(mine, all);
+  };
+  for (int t0 = 0; t0 < tiles; t0 += NT) {
+    measure(t0 + tid);
     sum += all;
   }
   AttendCursor c{0, 0, 0, 0, 0};
   line->total = sum * a.Hkv;
   line->used = min((int64_t)a.ctas, line->total);
-  int32_t* found = sh + 34;
+  int32_t* found = sh + 32;  // start: request, tile of it, tile of the head, place in the tile; end: the last two
   if ((int64_t)blockIdx.x < line->used) {  // the same for the whole CTA
-    const int64_t u0 = attend_div((int64_t)blockIdx.x * line->total, line->used);
-    const int64_t u1 = attend_div(((int64_t)blockIdx.x + 1) * line->total, line->used);
-    const int64_t h = attend_div(u0, sum), want = u0 - h * sum;
+    const int64_t x0 = attend_div((int64_t)blockIdx.x * line->total, line->used);
+    const int64_t x1 = attend_div(((int64_t)blockIdx.x + 1) * line->total, line->used);
+    const int64_t h0 = attend_div(x0, sum), h1 = attend_div(x1, sum);
+    const int64_t want0 = x0 - h0 * sum, want1 = x1 - h1 * sum;
     int64_t base = 0;
     for (int t0 = 0; t0 < tiles; t0 += NT) {
-      if (tiles > NT) {
-        const int t = t0 + tid;
-        mine = 0;
-        if (t < tiles) {
-          my_i = tile_of(t, my_r);
-          mine = attend_tile<KB>(a, my_r, my_i).units;
-        }
-        before = scan(mine, all);
-      }
-      if (base + before <= want && want < base + before + mine) {
+      const int t = t0 + tid;
+      if (tiles > NT) measure(t);
+      const int64_t at = base + before;
+      if (at <= want0 && want0 < at + mine) {
         found[0] = my_r;
         found[1] = my_i;
-        found[2] = (int)(want - base - before);
+        found[2] = t;
+        found[3] = (int)(want0 - at);
+      }
+      if (at <= want1 && want1 < at + mine) {
+        found[4] = t;
+        found[5] = (int)(want1 - at);
       }
       base += all;
-      if (base > want) break;
+      if (base > want0 && base > want1) break;
     }
     __syncthreads();
-    c = AttendCursor{(int)h, found[0], found[1], found[2], u1 - u0};
+    // units before a place: its distance, less the extra room of the tiles before it and of its own
+    const int64_t u0 = x0 - Extra * (h0 * tiles + found[2]) - min(found[3], Extra);
+    const int64_t u1 = x1 - Extra * (h1 * tiles + found[4]) - min(found[5], Extra);
+    c = AttendCursor{(int)h0, found[0], found[1], max(0, found[3] - Extra), u1 - u0};
   }
   __syncthreads();
   return c;

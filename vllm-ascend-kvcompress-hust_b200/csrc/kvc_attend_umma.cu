@@ -72,6 +72,10 @@ struct Geom {
   static constexpr int kFit = (225 * 1024 - NT * kQ) / kSlot;
   static constexpr int S = kFit > 10 ? 10 : kFit;
   static constexpr int OC = NT == 2 ? D : D / 2;   // O columns of a softmax thread
+  // Room of a tile on the line beside its units: cycles of its start and end (first loads, output) over those
+  // of a unit, 24,000 / 2,900, 25,000 / 3,900 and 7,000 / 3,400.  Against none: 12 ragged requests at 16 / 2 heads
+  // of 256 295 -> 274 us, an 8,191-token windowed prompt at 16 / 8 of 64 122 -> 115 us; doubled, 278 and 117.
+  static constexpr int kExtra = D == 256 ? 8 : D == 128 ? 6 : 2;
   // barriers, 8 bytes each: places in their array
   enum Bar : int { kFull = 0, kEmpty = S, kQFull = 2 * S, kQEmpty, kSFull, kPFull = kSFull + 4, kODone = kPFull + 4,
                    kSRead = kODone + 4, kOFree, kDone = kOFree + 2, kBars };
@@ -200,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
     tmem_relinquish();
   }
   AttendLine line;
-  AttendCursor c = attend_locate<KB, kThreads>(a, reinterpret_cast<int32_t*>(base + NT * G_::kQ), &line);
+  AttendCursor c = attend_locate<KB, kThreads, G_::kExtra>(a, reinterpret_cast<int32_t*>(base + NT * G_::kQ), &line);
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the ring held the prefix sums
   tc_fence_before();
   __syncthreads();
