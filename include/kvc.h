@@ -455,11 +455,12 @@ int kvc_rotary_write(const void* q, int64_t q_token_stride, int64_t q_head_strid
  * that no request owns are left as they were.  lse [num_tokens][heads] may be NULL.
  * max_query_len bounds the n; it picks the kernel, not the result.
  * Geometries: head_dim 64, 128 or 256, heads / kv_heads <= 16, up to 8192
- * requests.  Strides in elements, multiples of 8; pointers 16-byte aligned.
+ * requests, table_width up to 2^22.  Strides in elements, multiples of 8; pointers 16-byte aligned.
  * workspace: kvc_paged_attention_workspace_bytes, uninitialised; a call may
  * not share it with another that runs at the same time.  A block id outside
  * [0, num_blocks) or past table_width raises KVC_DEV_BLOCK_RANGE and its keys
- * count as unseen; query_start_loc entries that decrease or pass num_tokens
+ * count as unseen (a length far past the table costs one block's time); a
+ * negative length counts as 0; query_start_loc entries that decrease or pass num_tokens
  * raise KVC_DEV_INDEX_RANGE and leave that request out.
  */
 int64_t kvc_paged_attention_workspace_bytes(int max_query_len, int heads, int kv_heads, int head_dim);

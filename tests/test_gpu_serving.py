@@ -237,6 +237,17 @@ def test_many_requests_and_a_chunk_of_a_whole_prompt(dim):
     check_attention(c, attend(c, window=50, sinks=3), 50, 3)
 
 
+@pytest.mark.parametrize("longest,extra", [(1, 0), (3, 0), (1, 64), (150, 64)])
+def test_more_tiles_than_threads_of_a_block(longest, extra):
+    new = [(i * 7) % (longest + 1) if i % 50 == 3 else i % 3 != 0 for i in range(1100)]
+    new[-1] = longest
+    lens = [n + (53 * i) % 300 for i, n in enumerate(new)]
+    c = attention_case([int(n) for n in new], lens, 4, 2, 64, BF16)
+    kw = {"max_query_len": max(longest, extra)}  # 64: the kernel for chunks, whatever the lengths
+    check_attention(c, attend(c, **kw))
+    check_attention(c, attend(c, window=40, sinks=130, **kw), 40, 130)
+
+
 def test_rows_that_see_nothing_and_requests_without_keys():
     c = attention_case([1, 5, 1, 3], [0, 2, 7, -4], 8, 2, 128, BF16)
     out, lse = attend(c)
@@ -328,6 +339,25 @@ def test_bad_block_ids_and_row_ranges_are_flagged(new):
     out, _ = attend(far, error_flag=err)
     assert err.item() == N.DEV_INDEX_RANGE
     assert torch.equal(out[: new[0]], want[0][: new[0]])
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1, 1, 1], [9, 1, 50, 1, 3]])
+@pytest.mark.parametrize("window", [0, 60])
+def test_lengths_that_no_table_holds_are_flagged_and_leave_the_others(new, window):
+    top = 2 ** 31 - 1
+    for c, lens, rows in (
+            (attention_case(new, [300, 0, 200, 10, 129], 4, 2, 64, BF16), [300, top, 200, -top - 1, 129], (0, 2, 4)),
+            (attention_case([1] * 500 + [new[0]], [5] * 500 + [300], 4, 2, 64, BF16), [top] * 500 + [300], (500,))):
+        out, lse, ob, lb = R.attention(c["q"], c["kc"], c["vc"], c["table"], c["starts"], c["lens"], 64 ** -0.5, window, 0)
+        err = ints([0])
+        got, l = (x.double().cpu() for x in attend(dict(c, lens=lens), window=window, error_flag=err))
+        assert err.item() == N.DEV_BLOCK_RANGE
+        for r in rows:
+            s = slice(c["starts"][r], c["starts"][r + 1])
+            assert ((got[s] - out[s]).abs() <= ob[s]).all() and ((l[s] - lse[s]).abs() <= lb[s]).all()
+        for r in [r for r, n in enumerate(lens) if n < 0]:
+            s = slice(c["starts"][r], c["starts"][r + 1])
+            assert (got[s] == 0).all() and (l[s] == -math.inf).all()
 
 
 @pytest.mark.parametrize("new", [[1] * 5, [1, 200, 3, 1, 64]])

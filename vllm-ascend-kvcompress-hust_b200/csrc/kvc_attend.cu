@@ -570,7 +570,7 @@ extern "C" int kvc_paged_attention(const void* q, int64_t q_token_stride, int64_
                     window >= 0 && sinks >= 0 && scale > 0.f && scale <= 3.0e38f,
                 KVC_EINVAL);
   KVC_CHECK_ARG(heads / kv_heads <= kRows && (head_dim == 64 || head_dim == 128 || head_dim == 256) &&
-                    num_requests <= kMaxAttendRequests,
+                    num_requests <= kMaxAttendRequests && table_width <= kMaxAttendWidth,
                 KVC_EUNSUPPORTED);
   if (num_requests == 0 || num_tokens == 0 || max_query_len == 0) return KVC_OK;
   KVC_CHECK_ARG(q && k_cache && v_cache && query_start_loc && seq_lens && out && workspace &&

@@ -30,6 +30,7 @@ namespace kvc {
 
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr int kMaxAttendRequests = 8192;
+constexpr int kMaxAttendWidth = 1 << 22;  // entries of a table row: units of a block's threads stay within 32 bits
 
 struct AttendArgs {
   CUtensorMap kmap, vmap;  // [block][token][head][dim], boxes of 64 dims x KB tokens of one head
@@ -73,15 +74,16 @@ __device__ __forceinline__ AttendTile attend_tile(const AttendArgs& a, int r, in
   t.r = r;
   t.row0 = q0 + i * a.tok;
   t.ntok = min(a.tok, n - i * a.tok);
-  t.pos0 = __ldg(a.lens + r) - n + i * a.tok;
+  t.pos0 = max(__ldg(a.lens + r), 0) - n + i * a.tok;  // no keys: every row is before the first
   t.head_blocks = t.lo_block = 0;
   const int last = t.last();
+  const int past = a.table_width * (kBlock / KB);  // of the blocks past the table a tile has this one, which raises the error
   if (a.window > 0 && t.pos0 >= a.window) {
-    t.lo_block = (t.pos0 - a.window + 1) / KB;
+    t.lo_block = min((t.pos0 - a.window + 1) / KB, past);
     t.head_blocks = min((a.sinks + KB - 1) / KB, t.lo_block);
   }
   // a tile that sees nothing still has one unit, so that its rows are written
-  t.units = last < 0 ? 1 : t.head_blocks + last / KB - t.lo_block + 1;
+  t.units = last < 0 ? 1 : t.head_blocks + min(last / KB, past) - t.lo_block + 1;
   return t;
 }
 
