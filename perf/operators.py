@@ -11,7 +11,6 @@ Four operators, in the order a decode or chunked-prefill step runs them:
 ``own`` set, makes the framework's calls.
 """
 
-import functools
 import math
 import random
 import sys
@@ -301,8 +300,7 @@ def _plain_attend(s):
 # ---- the framework's calls -----------------------------------------------------------------------
 
 
-@functools.cache
-def _kernels():  # a program imports the framework once
+def _kernels():
     root = str(Path(__file__).resolve().parents[1] / "vllm-ascend-kvcompress-hust_b200")
     if root not in sys.path:
         sys.path.insert(0, root)
