@@ -78,7 +78,7 @@ struct Geom {
   static constexpr int kExtra = D == 256 ? 8 : D == 128 ? 6 : 2;
   // barriers, 8 bytes each: places in their array
   enum Bar : int { kFull = 0, kEmpty = S, kQFull = 2 * S, kQEmpty, kSFull, kPFull = kSFull + 4, kODone = kPFull + 4,
-                   kSRead = kODone + 4, kOFree, kDone = kOFree + 2, kBars };
+                   kSRead = kODone + 4, kOFree, kDone = kOFree + 2, kRead, kCleared, kBars };
   static constexpr int kTail = kBars * 8 + kMeta * 4 + 16 + (NT == 1 ? 2048 : 0);
   static constexpr int kSmem = NT * kQ + S * kSlot + kTail;
   static_assert(S >= 5 && kSmem <= 227 * 1024 && kSmem > 116 * 1024, "one CTA per SM: it holds every TMEM column");
@@ -119,8 +119,13 @@ __device__ __forceinline__ void tma_4d(uint32_t dst, const void* map, int c0, in
       : "memory");
 }
 
-__device__ __forceinline__ void named_sync(int threads) {
-  asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");
+// Named barriers.  With two halves a warpgroup may run ahead of the other by a tile, so each id has one set of
+// threads that ever comes to it, and what both have to meet for are mbarriers, whose waits are bounded: both
+// warpgroups (one half); each one's look at the values; a warpgroup by itself.
+constexpr int kBarBoth = 1, kBarLook = 2, kBarOwn = 4;
+
+__device__ __forceinline__ void named_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 __device__ __forceinline__ bool named_or(int id, int threads, bool x) {
   uint32_t y;
@@ -170,6 +175,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
   const uint32_t sread = full0 + 8 * G_::kSRead;  // S has been read (one half)
   const uint32_t ofree = full0 + 8 * G_::kOFree;  // [half] the tile's output has been read
   const uint32_t done = full0 + 8 * G_::kDone;    // every product is complete
+  const uint32_t vread = full0 + 8 * G_::kRead, vclear = full0 + 8 * G_::kCleared;  // a block's odd values (two halves)
   volatile uint32_t* meta = reinterpret_cast<uint32_t*>(bars + G_::kBars);  // per unit, from the producer
   uint32_t* tmem_slot = const_cast<uint32_t*>(meta + kMeta);
   float* xch = reinterpret_cast<float*>(tmem_slot + 4);  // [2][2][128] (NT == 1)
@@ -197,6 +203,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
     mbar_init(sread, 8);
     for (int i = 0; i < 2; ++i) mbar_init(ofree + 8 * i, NT == 2 ? 4 : 8);
     mbar_init(done, 2);
+    mbar_init(vread, 8);
+    mbar_init(vclear, 8);
     mbar_init_fence();
   }
   if (warp == kMma) {
@@ -432,6 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
     const uint32_t ocol = lane_base + G_::o_col(half) + (NT == 1 ? wg * OC : 0);
     const int tk = r / a.G;  // token of the half
     uint32_t g = 0, ga = 0;  // units of this half, and of the CTA
+    uint32_t odd_blocks = 0;  // that both halves have cleared
     bool dead = false;
     auto wait = [&](uint32_t bar, uint32_t parity) {
       if (!dead) dead = !mbar_wait_short(bar, parity, a.error_flag);
@@ -501,7 +510,18 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
                 odd |= odd_pair<FP16>(w[0]) | odd_pair<FP16>(w[1]) | odd_pair<FP16>(w[2]) | odd_pair<FP16>(w[3]);
               }
               const int team = NT == 1 || halves == 2 ? 256 : 128;
-              if (named_or(2 + (NT == 1 ? 0 : wg), kLook, odd)) {
+              auto meet = [&](uint32_t bar) {  // the team's warps; two halves' by mbarrier
+                if (NT == 1) {
+                  named_sync(kBarBoth, 256);
+                } else if (halves == 1) {
+                  named_sync(kBarOwn, 128);
+                } else {
+                  __syncwarp();
+                  if (lane == 0) mbar_arrive(bar);
+                  wait(bar, odd_blocks & 1);
+                }
+              };
+              if (named_or(kBarLook + (NT == 1 ? 0 : wg), kLook, odd)) {
                 const int d0 = NT == 1 ? wg * OC : 0;
                 if (live && !poison) {
                   for (int d = 0; d < OC; ++d) mine[d] = 0.f;
@@ -523,7 +543,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
                     if (!isfinite(v.y)) mine[d - d0 + 1] += v.y;
                   }
                 }
-                named_sync(team);  // read by all before it is cleared
+                meet(vread);  // read by all before it is cleared
                 for (int i = team == 256 ? tid : r; i < kVec; i += team) {
                   const uint32_t ad = vaddr(i);
                   uint32_t w[4];
@@ -537,7 +557,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                named_sync(team);
+                meet(vclear);
+                if (halves == 2) ++odd_blocks;
               }
             }
             tmem_ld_wait();
@@ -606,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
                 float mx = largest();
                 if constexpr (NT == 1) {
                   xch[((g & 1) * 2 + wg) * 128 + r] = mx;
-                  named_sync(256);
+                  named_sync(kBarBoth, 256);
                   mx = fmaxf(mx, xch[((g & 1) * 2 + (wg ^ 1)) * 128 + r]);
                 }
                 const bool raise = !(mx <= m) && (m == -INFINITY || !((mx - m) * a.scale_log2 <= kSlack));  // or NaN
@@ -627,11 +648,11 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
         }
         // ---- the piece's output ----
         if constexpr (NT == 1) {
-          named_sync(256);
+          named_sync(kBarBoth, 256);
           xch[wg * 128 + r] = l;
-          named_sync(256);
+          named_sync(kBarBoth, 256);
           l += xch[(wg ^ 1) * 128 + r];
-          named_sync(256);
+          named_sync(kBarBoth, 256);
         }
         wait_o(g, 0);
         const int head = c.h * a.G + r - tk * a.G;
