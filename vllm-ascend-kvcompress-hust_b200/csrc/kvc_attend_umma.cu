@@ -656,7 +656,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
         }
         wait_o(g, 0);
         const int head = c.h * a.G + r - tk * a.G;
-        if (m == -INFINITY) any = false, l = 0.f;  // a row that has seen nothing answers 0
+        // A row that has seen nothing answers 0.  The sum tells: NaN scores leave no maximum, but a NaN sum.
+        if (l == 0.f) any = false;
         const float inv = l == 0.f ? 0.f : 1.f / l;
         uint16_t* dst = a.out + (int64_t)(t.row0 + token) * a.o_tok + (int64_t)head * a.o_head + (NT == 1 ? wg * OC : 0);
 #pragma unroll 1
@@ -692,7 +693,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
         if (live && (NT == 2 || wg == 0)) {
           if (!(starts && ends)) a.part_ml[part * a.rows + token * a.G + r - tk * a.G] = make_float2(m, l);
           else if (a.lse)
-            a.lse[(int64_t)(t.row0 + token) * a.Hq + head] = m == -INFINITY ? -INFINITY : m * a.scale + logf(l);
+            a.lse[(int64_t)(t.row0 + token) * a.Hq + head] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
         }
         arrive(ofree + 8 * half);
       } else {
