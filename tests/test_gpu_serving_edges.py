@@ -78,3 +78,65 @@ def test_nan_scores_in_a_part_of_a_request_cut_over_the_gpu(longest):
     out, lse = (x.cpu() for x in attend(q, max_query_len=longest))
     assert out[1, 3].isnan().all() and lse[1, 3].isnan()
     assert out.isnan().sum() == 128 and lse.isnan().sum() == 1
+
+
+# ---- fp16 weights far below the largest ------------------------------------------------------------
+
+
+def bits_below(kind, n, g):
+    """log2 of each key's weight against the largest, as how far below it lies."""
+    i = torch.arange(n, dtype=torch.float64)
+    if kind == "spread":
+        return 40 * torch.rand(n, generator=g, dtype=torch.float64)
+    if kind == "rising":  # every part has a new maximum
+        return 60 * (1 - i / n)
+    if kind == "plateaus":  # 64 weights alike, then 64 that are 3 bits higher, over and over
+        return 3.0 * (7 - (i // 64) % 8) + 24.0 * (n - 1 - i).div(512, rounding_mode="floor")
+    far = torch.full((n,), float(kind), dtype=torch.float64)  # one strong first token, all others alike
+    far[0] = 0
+    return far
+
+
+@pytest.mark.parametrize("kind,n", [("0", 5000), ("12", 65536), ("20", 65536), ("25.1", 65536), ("25.1", 700), ("28", 65536),
+                                    ("spread", 20000), ("rising", 9000), ("plateaus", 4100)])
+@pytest.mark.parametrize("dim,new", [(64, 1), (128, 1), (256, 1), (64, 30), (128, 30), (256, 30)])
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+def test_many_small_weights_beside_a_strong_one(kind, n, dim, new, dtype):
+    """The first token's value is 0, so the others' weights are all of the output.  150 requests read one cache, so
+    that most are not cut into parts, each with a largest weight of its own.
+
+    Bound of an output, relative to sum w |v|: half a step of the type for each weight and for the output; products
+    and sums in fp32, of up to n / 16 terms one after another (2^-23 each); the exponential and the scores (here one
+    product of at most 60 bits, so 2^-23 * 60 of a weight, and 2^-18 for the rest).  And of weights under fp16's
+    normal range half of its smallest subnormal, 2^-25: 64 of them beside the first token, whose weight is 2^3 (128
+    beside 2^7 at head_dim 256), and any others as 2^9 of what they are against it, 2^-22 + n 2^-34 of the row's
+    sum; in blocks of mixed weights, which average 2^-10 at least, 2^-15 of it.
+    """
+    g = torch.Generator().manual_seed(n + dim)
+    heads, blocks = 4, -(-n // 128)
+    q = torch.zeros(new, heads, dim)
+    q[..., 3] = 4.0
+    q[:, 1, 3], q[:, 2, 3] = 3.0, 3.5
+    kc = torch.zeros(blocks * 128, dim)
+    kc[:n, 3] = (-bits_below(kind, n, g) * math.log(2) / 4).float()
+    vc = 0.5 + torch.rand(blocks * 128, dim, generator=g)
+    vc[0] = 0
+    q, kc, vc = (x.to(dtype).cuda() for x in (q, kc, vc))
+    many = 150
+    out, lse = attend({"q": q.repeat(many, 1, 1), "kc": kc.view(blocks, 128, 1, dim), "vc": vc.view(blocks, 128, 1, dim),
+                       "table": torch.arange(blocks, dtype=torch.int32).repeat(many, 1),
+                       "starts": [new * i for i in range(many + 1)], "lens": [n] * many, "longest": new}, scale=1.0)
+    out, lse = out.unflatten(0, (many, new)), lse.unflatten(0, (many, new))
+    score = (q[..., 3].double().flatten()[:, None] * kc[:n, 3].double()).unflatten(0, (new, heads))
+    last = torch.arange(n - new, n, device="cuda")[:, None, None]
+    score = score.masked_fill(torch.arange(n, device="cuda") > last, -math.inf)
+    w = torch.softmax(score, -1)
+    want = w @ vc[:n].double()
+    u = torch.finfo(dtype).eps / 2
+    bound = want * (2 * u + 60 * 2.0 ** -23 + 2.0 ** -18 + n / 16 * 2.0 ** -23)
+    coarse = 2.0 ** -22 + n * 2.0 ** -34 if kind[0].isdigit() else 2.0 ** -15
+    bound += (coarse if dtype == FP16 else 0) * vc[:n].double().amax(0) + torch.finfo(dtype).tiny * 2 * u
+    over = (out.double() - want).abs() - bound
+    assert (over <= 0).all(), f"{over.max().item():.3g} past its bound where {want.mean().item():.3g} is usual"
+    off = (lse.double() - torch.logsumexp(score, -1)).abs()
+    assert (off <= 2.0 ** -16 + n / 16 * 2.0 ** -23).all()

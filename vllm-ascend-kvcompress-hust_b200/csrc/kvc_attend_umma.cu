@@ -19,8 +19,7 @@
 //    N-major operand: nothing is transposed;
 //  * two softmax warpgroups: a thread owns one row, so maximum and sum need no
 //    exchange; S row from TMEM, masked, 2^(c s - c m), rounded to the cache's
-//    type (the instruction wants A and B alike; off by half a step of the
-//    weight at most, as the output's own rounding) and stored back as P.
+//    type (the instruction wants A and B alike) and stored back as P.
 // head_dim 64 and 128: a tile has two halves of 128 rows, one per warpgroup and
 // MMA lane, that share every K/V block.  S comes in parts of 64 keys with two
 // buffers to a half (P goes over the S it came from): the next part's S is
@@ -33,8 +32,19 @@
 // The maximum that the weights are taken with is raised only when it has to be:
 // when a part's own exceeds it by 2^8, which at head_dim 64 and 128 is looked at
 // only when the sum of 64 weights passes 2^15, so that most parts need no pass
-// over the scores for their maximum.  Weights above 1 lose nothing in fp32, bf16
-// or fp16, and the output in TMEM is rescaled in the first parts of a row alone.
+// over the scores for their maximum.  Weights above 1 lose nothing in fp32 or
+// bf16, and the output in TMEM is rescaled in the first parts of a row alone.
+//
+// Rounding of P: half a step of the weight at most in bf16, whose range is
+// fp32's, as the output's own rounding.  fp16 ends at 2^16 and loses bits below
+// 2^-14, so a weight at the maximum is 2^3 there (2^7 at head_dim 256), and 2^9
+// (2^10) once a block's weights have averaged less than 2^-10.  What rounding takes
+// from weights that are below the range all the same is 2^-15 of the row's sum at
+// most; against a maximum of 1, keys under 2^-25 vanished beside a sum that
+// counts them, which many keys behind one strong first token feel.  Not 2^10 from
+// the start: the running maximum then outgrew the type too often (178 us for 119
+// in a windowed 8,191-token prompt at head_dim 64).  The range costs that case 2 %
+// (117 us without), and up to a sixth where scores are spread over tens of bits.
 //
 // Every wait is bounded (KVC_DEV_TIMEOUT); a softmax warp whose wait ran out
 // goes on without waiting, so every named barrier is met, the other roles
@@ -58,8 +68,17 @@ static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * kLaunchRegs, "registers");
 constexpr int KB = 128;                 // keys per unit
 constexpr int kSpan = 64;               // elements of a 128-byte swizzle span
 constexpr int kMeta = 16;
-constexpr float kSlack = 8.f;           // a maximum is raised for scores this far above it (log2 of their weight)
-constexpr float kMost = 32768.f;        // and for 64 weights with a larger sum
+
+// log2 of the weights: at the maximum, at first and once others were small; of the largest that leave the maximum as
+// it is.  kMost: the sum of 64 that does, at head_dim 64 and 128; 64 of 2^kTop have to be within it.
+template <bool FP16, int NT>
+struct Lift {
+  static constexpr float kFirst = FP16 ? (NT == 2 ? 3.f : 7.f) : 0.f;
+  static constexpr float kSmall = FP16 ? (NT == 2 ? 9.f : 10.f) : 0.f;
+  static constexpr float kTop = FP16 ? (NT == 2 ? 9.f : 15.f) : 8.f;
+  static constexpr float kMost = FP16 ? 49152.f : 32768.f;
+};
+constexpr float kMean = 1.f / 1024.f;  // weights are small where they average less
 
 template <int D>
 struct Geom {
@@ -160,6 +179,7 @@ template <int D, bool FP16>
 __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_constant__ AttendArgs a) {
   using G_ = Geom<D>;
   using E = std::conditional_t<FP16, Fp16, Bf16>;
+  using Lift_ = Lift<FP16, G_::NT>;
   constexpr int NT = G_::NT, S = G_::S, HV = G_::HV, SK = G_::SK;
   pdl_wait();
   pdl_trigger();
@@ -474,6 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
         // positions of this half's rows
         const int pos_first = t.pos0 + half * a.sub, pos_last = min(t.last(), pos_first + a.sub - 1);
         float m = -INFINITY, l = 0.f;
+        float base = -Lift_::kFirst;  // weights are 2^(c s - c m - base)
         bool any = false;     // a unit of the piece has been multiplied
         bool poison = false;  // `mine` holds infinite and NaN values to add to the output
         bool ready = false;   // every row of the warp has a maximum
@@ -572,7 +593,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
               // weights of the 64 keys, rounded into p; returns the sum of the unrounded ones
               uint32_t p[32];
               auto weigh = [&]() {
-                const float ms = m == -INFINITY ? 0.f : m * a.scale_log2;
+                const float ms = m == -INFINITY ? 0.f : FP16 ? fmaf(m, a.scale_log2, base) : m * a.scale_log2;
                 const float2 c2 = make_float2(a.scale_log2, a.scale_log2), n2 = make_float2(-ms, -ms);
                 float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
@@ -615,7 +636,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
               const bool seen = whole || attend_whole(a, pos_first, pos_last, k0 + 64 * part, 64);  // by this half's rows
               if (NT == 2 && seen && ready) {
                 sum = weigh();
-                fine = __all_sync(0xffffffffu, !live || sum <= kMost);
+                fine = __all_sync(0xffffffffu,
+                                  !live || (sum <= Lift_::kMost && (!FP16 || base != -Lift_::kFirst || sum >= 64.f * kMean)));
               }
               if (__builtin_expect(!fine, 0)) {
                 if (!seen) {
@@ -630,12 +652,27 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
                   named_sync(kBarBoth, 256);
                   mx = fmaxf(mx, xch[((g & 1) * 2 + (wg ^ 1)) * 128 + r]);
                 }
-                const bool raise = !(mx <= m) && (m == -INFINITY || !((mx - m) * a.scale_log2 <= kSlack));  // or NaN
-                const float f = raise && m > -INFINITY ? exp2_approx((m - mx) * a.scale_log2) : 1.f;
-                if (raise) m = mx;
+                const float top = (mx - m) * a.scale_log2 - base;  // log2 of the largest weight
+                float f = 1.f;
+                if (!(mx <= m) && m == -INFINITY) {
+                  m = mx;
+                } else if (FP16 ? top > Lift_::kTop : !(mx <= m) && !(top <= Lift_::kTop)) {
+                  f = exp2_approx((m - mx) * a.scale_log2);
+                  m = mx;
+                } else if (FP16 && base == -Lift_::kFirst) {
+                  // keys of the part (with one half, of the block) that the row sees
+                  const int c0 = k0 + (NT == 2 ? 64 * part : 0), lo = a.window > 0 ? pos - c0 - a.window : -1;
+                  const int hi = min(pos - c0, NT == 2 ? 63 : KB - 1);
+                  const int n = max(0, hi - max(lo, -1)) + max(0, min(min(a.sinks - c0 - 1, lo), hi) + 1);
+                  if (exp2_approx(top) < n * kMean) {
+                    f = (float)(1 << (int)(Lift_::kSmall - Lift_::kFirst));
+                    base = -Lift_::kSmall;
+                  }
+                }
                 if (__any_sync(0xffffffffu, f != 1.f)) rescale(f);
                 sum = weigh();
-                if (live && !(sum <= kMost)) sum = NAN;  // a score is infinite or NaN
+                // 64 of the largest weights and as much again for the rounding of large scores
+                if (live && !(sum <= (FP16 ? 4194304.f : 32768.f))) sum = NAN;  // a score is infinite or NaN
                 ready = __all_sync(0xffffffffu, !live || m > -INFINITY);
               }
               l += sum;
@@ -659,6 +696,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
         // A row that has seen nothing answers 0.  The sum tells: NaN scores leave no maximum, but a NaN sum.
         if (l == 0.f) any = false;
         const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float unit = FP16 ? __int_as_float((127 + (int)base) << 23) : 1.f;  // 2^base, for parts and lse
+        l *= unit;
         uint16_t* dst = a.out + (int64_t)(t.row0 + token) * a.o_tok + (int64_t)head * a.o_head + (NT == 1 ? wg * OC : 0);
 #pragma unroll 1
         for (int i = 0; i < OC; i += 32) {
@@ -681,6 +720,10 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
                   make_uint4(pack<FP16>(x[j], x[j + 1]), pack<FP16>(x[j + 2], x[j + 3]), pack<FP16>(x[j + 4], x[j + 5]),
                              pack<FP16>(x[j + 6], x[j + 7]));
           } else {
+            if constexpr (FP16) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) x[j] *= unit;
+            }
             if (poison) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) x[j] += mine[i + j];
