@@ -453,7 +453,8 @@ int kvc_rotary_write(const void* q, int64_t q_token_stride, int64_t q_head_strid
  * A row that sees no key (p < 0) gets 0 and -inf.  Keys and values that a row
  * does not see have no part in it, infinite and NaN ones included.  Rows of q
  * that no request owns are left as they were.  lse [num_tokens][heads] may be NULL.
- * max_query_len bounds the n; it picks the kernel, not the result.
+ * max_query_len bounds the n; it picks the kernel, not the result, except that 0
+ * says that no request has new tokens: nothing is launched.
  * Geometries: head_dim 64, 128 or 256, heads / kv_heads <= 16, up to 8192
  * requests, table_width up to 2^22.  Strides in elements, multiples of 8; pointers 16-byte aligned.
  * workspace: kvc_paged_attention_workspace_bytes, uninitialised; a call may

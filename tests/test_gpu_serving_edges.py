@@ -140,3 +140,16 @@ def test_many_small_weights_beside_a_strong_one(kind, n, dim, new, dtype):
     assert (over <= 0).all(), f"{over.max().item():.3g} past its bound where {want.mean().item():.3g} is usual"
     off = (lse.double() - torch.logsumexp(score, -1)).abs()
     assert (off <= 2.0 ** -16 + n / 16 * 2.0 ** -23).all()
+
+
+# ---- bounds and counts that are wrong --------------------------------------------------------------
+
+
+@pytest.mark.parametrize("new", [[1, 5, 0, 40], [1, 1, 1, 1]])
+def test_a_longest_length_of_zero_still_serves_the_tokens(new):
+    c = attention_case(new, [300, 900, 7, 40], 10, 2, 128, BF16)
+    want = attend(c, max_query_len=1)
+    out = torch.full(c["q"].shape, 7.0, dtype=BF16, device="cuda")
+    got = attend(c, max_query_len=0, out=out)
+    check_attention(c, got)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

@@ -646,7 +646,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``step_tables`` makes them).  A token at physical position p sees keys up
     to p; with ``window`` > 0 only the last ``window`` of them and the first
     ``sinks`` tokens of the cache.  ``scale`` defaults to ``dim ** -0.5``.
-    ``max_query_len`` is the most new tokens of a request.  Returns ``out``
+    ``max_query_len`` is the most new tokens of a request (it picks the kernel;
+    a wrong one costs time, not results).  Returns ``out``
     [N, heads, dim], or ``(out, lse)`` with the fp32 logarithm of each row's sum
     of exponentials.  ``workspace`` (``paged_attention_workspace_bytes``) is
     allocated per call unless given; one given must not serve two calls that
@@ -674,6 +675,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     qs, os = q.stride(), out.stride()
     if qs[2] != 1 or os[2] != 1:
         raise RuntimeError("q and out must have a contiguous last dim")
+    max_query_len = max_query_len or 1  # the C entry takes 0 for a step without tokens
     lse = torch.empty(n, heads, dtype=torch.float32, device=device) if return_lse else None
     if workspace is None:
         size = N.lib().kvc_paged_attention_workspace_bytes(max_query_len, heads, kvh, dim)
