@@ -393,7 +393,7 @@ int kvc_stage_commit(const int64_t* dst_blocks, const int64_t* dst_block_off, in
  * ones and offsets[r] tokens removed by compression (offsets NULL: none), and
  * page_table row r (page_stride elements apart, page_width entries) names its
  * scheduler pages of P = 128 * blocks_per_page tokens.
- *   query_start_loc [R + 1]  prefix sums of scheduled
+ *   query_start_loc [R + 1]  prefix sums of scheduled (2^31 - 1 where they pass it)
  *   seq_lens [R]             computed + scheduled - offset (physical)
  *   per token t < num_tokens of request r, j = t - query_start_loc[r]:
  *     positions[t] = computed[r] + j (semantic, for RoPE), request_indices[t] = r,

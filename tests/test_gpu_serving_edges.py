@@ -7,8 +7,9 @@ import math
 import pytest
 import torch
 
-import serving_reference as R
-from test_gpu_serving import BF16, FP16, attend, attention_case, check_attention, ints  # noqa: F401
+from test_gpu_serving import BF16, FP16, attend, attention_case, check_attention, ints
+from vllm_ascend_kvcompress import _native as N
+from vllm_ascend_kvcompress.methods.triattention import kernels as K
 
 pytestmark = pytest.mark.gpu
 
@@ -153,3 +154,26 @@ def test_a_longest_length_of_zero_still_serves_the_tokens(new):
     got = attend(c, max_query_len=0, out=out)
     check_attention(c, got)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+TOP = 2 ** 31 - 1
+
+
+def step(computed, scheduled, pages, num_tokens=4, max_blocks=3, page_dtype=torch.int32, **kw):
+    err = ints([0])
+    t = K.step_tables(ints(computed, torch.int64), ints(scheduled), torch.tensor(pages).to("cuda", page_dtype),
+                      num_tokens=num_tokens, max_blocks=max_blocks, error_flag=err, **kw)
+    return t, err.item()
+
+
+@pytest.mark.parametrize("scheduled", [[TOP, TOP, 4], [2, TOP, TOP, 2], [1] + [1 << 24] * 256 + [1], [1, 1, TOP] * 200])
+def test_counts_whose_sum_passes_32_bits_are_flagged_and_stay_in_order(scheduled):
+    requests = len(scheduled)
+    t, err = step([0] * requests, scheduled, [[3 + r % 2, 9] for r in range(requests)])
+    assert err & N.DEV_TOKEN_RANGE
+    starts = [min(sum(scheduled[:r]), TOP) for r in range(requests + 1)]
+    assert t.query_start_loc.tolist() == starts
+    first = [next(r for r in range(requests) if starts[r] <= i < starts[r + 1]) for i in range(4)]
+    assert t.request_indices.tolist() == first
+    assert t.positions.tolist() == [i - starts[r] for i, r in enumerate(first)]
+    assert t.slot_mapping.tolist() == [(3 + r % 2) * 128 + i - starts[r] for i, r in enumerate(first)]

@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const TablesArgs 
   kvc::pdl_wait();
   kvc::pdl_trigger();
   extern __shared__ int32_t start[];  // [R + 1] (token CTAs)
-  __shared__ int32_t warp_total[kThreads / 32];
+  __shared__ int64_t warp_total[kThreads / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
   if ((int)blockIdx.x >= a.token_ctas) {
@@ -99,30 +99,32 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const TablesArgs 
   }
 
   // ---- prefix sums of the new tokens ----
+  // In 64 bits: counts may add up to more than an int32.  Starts past one are kept as INT32_MAX, which no token
+  // reaches, so that they stay in order.
   int64_t carry = 0;
   for (int r0 = 0; r0 < a.R; r0 += kThreads) {
     const int r = r0 + tid;
     const int n = r < a.R ? new_tokens(a, r) : 0;
-    int v = n;
+    int64_t v = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, v, o);
+      const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
       if (lane >= o) v += u;
     }
     if (lane == 31) warp_total[warp] = v;
     __syncthreads();
-    int before = 0, all = 0;
+    int64_t before = 0, all = 0;
 #pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) {
-      const int t = warp_total[w];
+      const int64_t t = warp_total[w];
       if (w < warp) before += t;
       all += t;
     }
-    if (r < a.R) start[r] = (int32_t)(carry + before + v - n);
+    if (r < a.R) start[r] = (int32_t)kvc::min64(carry + before + v - n, INT32_MAX);
     carry += all;
     __syncthreads();
   }
-  if (tid == 0) start[a.R] = (int32_t)carry;
+  if (tid == 0) start[a.R] = (int32_t)kvc::min64(carry, INT32_MAX);
   __syncthreads();
   const int64_t total = carry;
   if (blockIdx.x == 0) {
