@@ -402,7 +402,8 @@ int kvc_stage_commit(const int64_t* dst_blocks, const int64_t* dst_block_off, in
  * num_tokens is the length of the per-token arrays; entries past the step's
  * last token get position 0, slot -1 and request -1.  computed, scheduled and
  * page_table hold 4- or 8-byte integers (*_bytes).  A page that the table lacks
- * (past page_width, or negative) raises KVC_DEV_BLOCK_RANGE and gives -1; a
+ * (past page_width, negative, or whose blocks pass an int32 or slots an int64)
+ * raises KVC_DEV_BLOCK_RANGE and gives -1; a
  * negative count, length or physical position, or more new tokens than
  * num_tokens, raises KVC_DEV_TOKEN_RANGE; more blocks than max_blocks raise
  * KVC_DEV_BLOCK_RANGE.  Up to 8192 requests.

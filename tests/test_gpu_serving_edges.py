@@ -177,3 +177,17 @@ def test_counts_whose_sum_passes_32_bits_are_flagged_and_stay_in_order(scheduled
     assert t.request_indices.tolist() == first
     assert t.positions.tolist() == [i - starts[r] for i, r in enumerate(first)]
     assert t.slot_mapping.tolist() == [(3 + r % 2) * 128 + i - starts[r] for i, r in enumerate(first)]
+
+
+@pytest.mark.parametrize("bpp,page,block,slot", [
+    (4, 1 << 62, -1, -1),                        # 4 * 2^62 is 0 in 64 bits
+    (16, (1 << 60) + 5, -1, -1),
+    (1, (1 << 56) + 7, -1, -1),                  # a slot of 2^63 and more
+    (1, 1 << 40, -1, (1 << 47) + 10),            # a slot that 64 bits hold, a block that an int32 does not
+    (2, 1 << 30, -1, (1 << 38) + 10),
+    (2, (1 << 30) - 1, (1 << 31) - 2, ((1 << 30) - 1) * 256 + 10),  # the last page whose blocks an int32 holds
+])
+def test_page_ids_past_the_range_are_flagged(bpp, page, block, slot):
+    t, err = step([10], [1], [[page]], num_tokens=1, max_blocks=1, page_dtype=torch.int64, blocks_per_page=bpp)
+    assert t.block_table.tolist() == [[block]] and t.slot_mapping.tolist() == [slot]
+    assert err == (0 if block >= 0 else N.DEV_BLOCK_RANGE)

@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const TablesArgs 
     if ((int64_t)b * kvc::kBlock < len) {
       const int page = b / a.bpp;
       if (page < a.page_width) id = a.pages[r * a.page_stride + page];
-      id = id < 0 ? -1 : id * a.bpp + b % a.bpp;
+      id = id < 0 || id > INT32_MAX ? -1 : id * a.bpp + b % a.bpp;  // below 2^62
       if (id < 0 || id > INT32_MAX) {
         kvc::raise_flag(a.error_flag, KVC_DEV_BLOCK_RANGE);
         id = -1;
@@ -135,6 +135,7 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const TablesArgs 
 
   // ---- one token per thread ----
   const int64_t page_tokens = (int64_t)kvc::kBlock * a.bpp;
+  const int64_t last_page = INT64_MAX / page_tokens - 1;  // whose slots are within 64 bits
   for (int64_t t = (int64_t)blockIdx.x * kThreads + tid; t < a.num_tokens; t += (int64_t)a.token_ctas * kThreads) {
     if (t >= total) {  // padding of a captured step: no request, no slot
       a.positions[t] = 0;
@@ -155,7 +156,7 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const TablesArgs 
       kvc::raise_flag(a.error_flag, KVC_DEV_TOKEN_RANGE);
     } else {
       const int64_t id = page < a.page_width ? a.pages[lo * a.page_stride + page] : -1;
-      if (id < 0) kvc::raise_flag(a.error_flag, KVC_DEV_BLOCK_RANGE);
+      if (id < 0 || id > last_page) kvc::raise_flag(a.error_flag, KVC_DEV_BLOCK_RANGE);
       else slot = id * page_tokens + (phys - page * page_tokens);
     }
     a.positions[t] = pos;
