@@ -463,7 +463,8 @@ int kvc_rotary_write(const void* q, int64_t q_token_stride, int64_t q_head_strid
  * [0, num_blocks) or past table_width raises KVC_DEV_BLOCK_RANGE and its keys
  * count as unseen (a length far past the table costs one block's time); a
  * negative length counts as 0; query_start_loc entries that decrease or pass num_tokens
- * raise KVC_DEV_INDEX_RANGE and leave that request out.
+ * raise KVC_DEV_INDEX_RANGE and leave that request out, and all of them where the
+ * others name rows so often that they have more tiles than there are rows and requests.
  */
 int64_t kvc_paged_attention_workspace_bytes(int max_query_len, int heads, int kv_heads, int head_dim);
 int kvc_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int dtype,

@@ -191,3 +191,20 @@ def test_page_ids_past_the_range_are_flagged(bpp, page, block, slot):
     t, err = step([10], [1], [[page]], num_tokens=1, max_blocks=1, page_dtype=torch.int64, blocks_per_page=bpp)
     assert t.block_table.tolist() == [[block]] and t.slot_mapping.tolist() == [slot]
     assert err == (0 if block >= 0 else N.DEV_BLOCK_RANGE)
+
+
+@pytest.mark.parametrize("longest", [1, 64])
+@pytest.mark.parametrize("tail", [[0], [0, 3]])
+def test_starts_that_name_the_rows_thousands_of_times_are_flagged(longest, tail):
+    """4,096 requests of 2^20 rows each: 2^32 rows, as starts that go back and forth name them."""
+    n = 1 << 20
+    starts = ([0, n] * 4096 + tail)[: 8193]
+    memory = [torch.full((8 * n + 16 * 64,), 3.0, dtype=BF16, device="cuda") for _ in range(2)]  # rows overlap: 16 MB
+    q, out = (x.as_strided((n, 16, 64), (8, 64, 1)) for x in memory)
+    cache = torch.zeros(1, 128, 1, 64, dtype=BF16, device="cuda")
+    requests = len(starts) - 1
+    err = ints([0])
+    K.paged_attention(q, cache, cache, torch.zeros(requests, 1, dtype=torch.int32, device="cuda"), ints(starts),
+                      ints([5] * requests), max_query_len=longest, out=out, error_flag=err)
+    assert err.item() == N.DEV_INDEX_RANGE
+    assert (memory[1] == 3.0).all()

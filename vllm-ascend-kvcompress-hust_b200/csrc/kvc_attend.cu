@@ -61,7 +61,7 @@ struct Geom {
   static constexpr int kKeys = KB / kConsumers;    // keys per warp and unit
   static constexpr int kSmem = kStages * kStage + kMerge + kTail;
   static_assert(kStages >= 2 && kSmem <= 227 * 1024, "shared memory");
-  static_assert(kStages * kStage >= (kMaxAttendRequests + 41) * 4, "the prefix sums lie in the stages");
+  static_assert(kStages * kStage >= (kMaxAttendRequests + 1 + kLocateInts) * 4, "the prefix sums lie in the stages");
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {

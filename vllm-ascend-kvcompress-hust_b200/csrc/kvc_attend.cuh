@@ -117,43 +117,54 @@ __device__ __forceinline__ int64_t attend_owner(const AttendLine& l, int64_t x) 
   return attend_div((x + 1) * l.used - 1, l.total);
 }
 
-// All threads: this CTA's piece of the line.  `sh`: R + 1 + 40 ints of shared memory, free again on return.
+constexpr int kLocateInts = 72;  // shared memory of attend_locate beside the R + 1 prefix sums, in ints
+
+// All threads: this CTA's piece of the line.  `sh`: kLocateInts + R + 1 ints of shared memory, free again on return.
 template <int KB, int NT, int Extra>
 __device__ AttendCursor attend_locate(const AttendArgs& a, int32_t* sh, AttendLine* line) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int32_t* first = sh + 40;  // [R + 1] tiles before each request
+  int32_t* first = sh + kLocateInts;  // [R + 1] tiles before each request
   constexpr int kWarps = NT / 32;
   static_assert(kWarps <= 32, "");
-  auto scan = [&](int n, int& all) {  // exclusive prefix of n over the threads
-    int v = n;
+  auto scan = [&](auto n, auto& all) {  // exclusive prefix of n over the threads
+    using T = decltype(n);
+    T* totals = reinterpret_cast<T*>(sh);  // [32]
+    T v = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, v, o);
+      const T u = __shfl_up_sync(0xffffffffu, v, o);
       if (lane >= o) v += u;
     }
     __syncthreads();
-    if (lane == 31) sh[warp] = v;
+    if (lane == 31) totals[warp] = v;
     __syncthreads();
-    int before = 0;
+    T before = 0;
     all = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const int t = sh[w];
+      const T t = totals[w];
       if (w < warp) before += t;
       all += t;
     }
     return before + v - n;
   };
-  int carry = 0, all = 0;
+  // In 64 bits: starts that go back can name q's rows any number of times.  Requests with rows of their own have no
+  // more tiles than rows, and with more than that and one for each request none is served.
+  int64_t carry = 0, some = 0;
   for (int r0 = 0; r0 < a.R; r0 += NT) {
-    const int r = r0 + tid, n = r < a.R ? attend_tiles(a, r) : 0;
-    const int before = scan(n, all);
-    if (r < a.R) first[r] = carry + before;
-    carry += all;
+    const int r = r0 + tid;
+    const int64_t before = scan((int64_t)(r < a.R ? attend_tiles(a, r) : 0), some);
+    if (r < a.R) first[r] = (int32_t)min64(carry + before, INT32_MAX);
+    carry += some;
   }
-  if (tid == 0) first[a.R] = carry;
+  if (carry > min64(a.num_tokens + a.R, INT32_MAX)) {
+    raise_flag(a.error_flag, KVC_DEV_INDEX_RANGE);
+    carry = 0;
+  }
+  if (tid == 0) first[a.R] = (int32_t)carry;
   __syncthreads();
-  const int tiles = carry;
+  const int tiles = (int)carry;
+  int all = 0;
   auto tile_of = [&](int t, int& r) {  // request of tile t: the last that starts at or before it
     int lo = 0, hi = a.R - 1;
     while (lo < hi) {
@@ -181,7 +192,7 @@ __device__ AttendCursor attend_locate(const AttendArgs& a, int32_t* sh, AttendLi
   AttendCursor c{0, 0, 0, 0, 0};
   line->total = sum * a.Hkv;
   line->used = min((int64_t)a.ctas, line->total);
-  int32_t* found = sh + 32;  // start: request, tile of it, tile of the head, place in the tile; end: the last two
+  int32_t* found = sh + 64;  // start: request, tile of it, tile of the head, place in the tile; end: the last two
   if ((int64_t)blockIdx.x < line->used) {  // the same for the whole CTA
     const int64_t x0 = attend_div((int64_t)blockIdx.x * line->total, line->used);
     const int64_t x1 = attend_div(((int64_t)blockIdx.x + 1) * line->total, line->used);

@@ -101,7 +101,7 @@ struct Geom {
   static constexpr int kTail = kBars * 8 + kMeta * 4 + 16 + (NT == 1 ? 2048 : 0);
   static constexpr int kSmem = NT * kQ + S * kSlot + kTail;
   static_assert(S >= 5 && kSmem <= 227 * 1024 && kSmem > 116 * 1024, "one CTA per SM: it holds every TMEM column");
-  static_assert(S * kSlot >= (kMaxAttendRequests + 41) * 4, "the prefix sums lie in the ring");
+  static_assert(S * kSlot >= (kMaxAttendRequests + 1 + kLocateInts) * 4, "the prefix sums lie in the ring");
   // TMEM columns.  Two halves: S of a half's 64-key parts, P over the S it came from.  One: S of 128 keys, P
   // of even and odd units.  O from 256 on.
   static __device__ __forceinline__ uint32_t s_col(int half, int part) { return 128 * half + 64 * part; }
