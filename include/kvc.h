@@ -406,7 +406,10 @@ int kvc_stage_commit(const int64_t* dst_blocks, const int64_t* dst_block_off, in
  * raises KVC_DEV_BLOCK_RANGE and gives -1; a
  * negative count, length or physical position, or more new tokens than
  * num_tokens, raises KVC_DEV_TOKEN_RANGE; more blocks than max_blocks raise
- * KVC_DEV_BLOCK_RANGE.  Up to 8192 requests.
+ * KVC_DEV_BLOCK_RANGE (max_blocks 0: no block table is wanted, and none is looked
+ * at).  Up to 8192 requests.  No table may share memory with another or with an
+ * input (KVC_EINVAL): lengths of an earlier call are copied before they become
+ * this one's, or its tables written to a second set.
  */
 int kvc_step_tables(const void* computed, int computed_bytes, const void* scheduled, int scheduled_bytes,
                     const int64_t* offsets, int num_requests, const void* page_table, int page_bytes,

@@ -208,3 +208,20 @@ def test_starts_that_name_the_rows_thousands_of_times_are_flagged(longest, tail)
                       ints([5] * requests), max_query_len=longest, out=out, error_flag=err)
     assert err.item() == N.DEV_INDEX_RANGE
     assert (memory[1] == 3.0).all()
+
+
+def test_tables_that_are_also_inputs_are_refused():
+    t, err = step([10, 300], [1, 1], [[0, 1, 2], [3, 4, 5]], num_tokens=2)
+    assert err == 0
+    pages = ints([[0, 1, 2], [3, 4, 5]])
+    with pytest.raises(RuntimeError, match="kvc_step_tables"):  # the last step's lengths, and its tables again
+        K.step_tables(t.seq_lens, ints([1, 1]), pages, num_tokens=2, max_blocks=3, out=t)
+    with pytest.raises(RuntimeError, match="kvc_step_tables"):
+        K.step_tables(ints([11, 301]), ints([1, 1]), t.block_table, num_tokens=2, max_blocks=3, out=t)
+    with pytest.raises(RuntimeError, match="kvc_step_tables"):
+        K.step_tables(ints([11, 301]), ints([1, 1]), pages, num_tokens=2, max_blocks=3, out=t._replace(slot_mapping=t.positions))
+    both = torch.arange(2, device="cuda", dtype=torch.int32)  # inputs alone may
+    u = K.step_tables(both, both, pages, num_tokens=2, max_blocks=3, out=t)
+    assert u.query_start_loc.tolist() == [0, 0, 1] and u.seq_lens.tolist() == [0, 2]
+    v = K.step_tables(u.seq_lens, ints([1, 1]), pages, num_tokens=2, max_blocks=3)  # into tables of its own
+    assert v.seq_lens.tolist() == [1, 3]

@@ -165,6 +165,16 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const TablesArgs 
   }
 }
 
+struct Range {
+  const void* p;
+  int64_t bytes;
+};
+
+bool overlap(const Range& a, const Range& b) {
+  const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+  return a.bytes > 0 && b.bytes > 0 && x < y + (uintptr_t)b.bytes && y < x + (uintptr_t)a.bytes;
+}
+
 }  // namespace
 
 extern "C" int kvc_step_tables(const void* computed, int computed_bytes, const void* scheduled, int scheduled_bytes,
@@ -183,6 +193,18 @@ extern "C" int kvc_step_tables(const void* computed, int computed_bytes, const v
                     (page_bytes == 4 || page_bytes == 8),
                 KVC_EINVAL);
   KVC_CHECK_ARG(num_requests <= kMaxRequests, KVC_EUNSUPPORTED);
+  // CTAs read the inputs while others write tables: lengths of an earlier call, say, cannot be both
+  const int64_t R = num_requests, N = num_tokens;
+  const Range read[] = {{computed, R * computed_bytes},
+                        {scheduled, R * scheduled_bytes},
+                        {offsets, offsets ? 8 * R : 0},
+                        {page_table, ((R - 1) * page_stride + page_width) * page_bytes}};
+  const Range written[] = {{query_start_loc, 4 * (R + 1)}, {seq_lens, 4 * R},        {positions, 8 * N},
+                           {slot_mapping, 8 * N},          {request_indices, 4 * N}, {block_table, 4 * R * max_blocks}};
+  for (const Range& w : written) {
+    for (const Range& r : read) KVC_CHECK_ARG(!overlap(w, r), KVC_EINVAL);
+    for (const Range& o : written) KVC_CHECK_ARG(&o == &w || !overlap(w, o), KVC_EINVAL);
+  }
   TablesArgs a{};
   a.computed = {computed, computed_bytes};
   a.scheduled = {scheduled, scheduled_bytes};

@@ -535,7 +535,8 @@ def step_tables(computed: torch.Tensor, scheduled: torch.Tensor, page_table: tor
     per-token tables (the step's new tokens, or more in a captured step: entries
     past the last token get slot and request -1) and ``max_blocks`` the width of
     the block table, whose entries past a request's blocks are -1.  ``out``
-    takes tables of an earlier call or ``StepTables.empty``.
+    takes tables of an earlier call or ``StepTables.empty``; none of them may
+    share memory with an input (a last step's ``seq_lens`` as ``computed``, say).
     """
     device = _device_of(computed, scheduled, page_table, offsets, error_flag)
     R = computed.numel()
