@@ -225,3 +225,39 @@ def test_tables_that_are_also_inputs_are_refused():
     assert u.query_start_loc.tolist() == [0, 0, 1] and u.seq_lens.tolist() == [0, 2]
     v = K.step_tables(u.seq_lens, ints([1, 1]), pages, num_tokens=2, max_blocks=3)  # into tables of its own
     assert v.seq_lens.tolist() == [1, 3]
+
+
+@pytest.mark.parametrize("size", [2.0 ** 12, 2.0 ** 20, 2.0 ** 24, 2.0 ** 26])
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+@pytest.mark.parametrize("dim,longest", [(64, 1), (128, 1), (256, 1), (64, 64), (128, 64), (256, 64)])
+def test_scores_whose_rounding_is_bits(size, dtype, dim, longest):
+    """Scores near `size` that differ by small whole numbers answer a mean of the values, never inf or NaN.
+
+    The scores are exact here (two products of powers of two and small integers; at 2^24 and past it the integers
+    are multiples of the step).  A maximum in units of log2 rounds by up to 2^-24 of itself, which moves all weights
+    taken with it by as many bits; parts that were taken with two of them are up to twice as far apart, so the
+    weights of a mean are each within a factor 2^s and the mean within 2^2s, and never outside the values.
+    """
+    n, heads = 600, 4
+    step = max(1.0, size * 2.0 ** -23)
+    g = torch.Generator().manual_seed(dim)
+    below = step * torch.randint(0, 7, (n,), generator=g).float()
+    half = size ** 0.5 if math.log2(size) % 2 == 0 else None
+    q, k = torch.zeros(3, heads, dim), torch.zeros(640, dim)
+    q[..., 0], k[:, 0] = half, half
+    q[..., 9], k[:n, 9] = step, -below / step
+    v = 0.5 + torch.rand(640, dim, generator=g)
+    q, k, v = (x.to(dtype) for x in (q, k, v))
+    assert q[0, 0, 0] == half and k[0, 0] == half and (k[:n, 9].float() == -below / step).all()
+    out, lse = attend({"q": q, "kc": k.view(5, 128, 1, dim), "vc": v.view(5, 128, 1, dim),
+                       "table": torch.arange(5, dtype=torch.int32).repeat(3, 1), "starts": [0, 1, 2, 3],
+                       "lens": [n] * 3, "longest": longest}, scale=1.0)
+    w = torch.softmax(-below.double(), 0)
+    want = w @ v[:n].double()
+    u = torch.finfo(dtype).eps / 2
+    s = 2 * size * math.log2(math.e) * 2.0 ** -24
+    out = out.double().cpu()
+    top, bottom = v[:n].double().amax(0), v[:n].double().amin(0)
+    assert (out <= top * (1 + 2 * u + 2.0 ** -18)).all() and (out >= bottom * (1 - 2 * u - 2.0 ** -18)).all()
+    assert ((out - want).abs() <= want * (2 * u + 2.0 ** -18 + 4.0 ** s - 1)).all()
+    assert (lse.double().cpu() - size).abs().max() <= 8 + size * 2.0 ** -21

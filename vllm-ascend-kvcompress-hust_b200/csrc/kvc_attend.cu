@@ -23,7 +23,7 @@
 // instruction wants both operands alike.  In bf16, whose range is fp32's, each
 // weight is off by half a step at most (2^-8 of it), independent from key to key,
 // which is no more than the output's own rounding.  In fp16 the weights are taken
-// kLift<true> bits higher than against a maximum of 1: half a step (2^-11 of it)
+// 14 bits higher than against a maximum of 1 (lift_of): half a step (2^-11 of it)
 // for weights down to 2^-28 of the row's largest, and 2^-39 of the largest for
 // those below; against 1, weights under 2^-25 would vanish beside a sum that
 // counts them, which many keys behind one strong first token feel.
@@ -42,10 +42,13 @@ constexpr int kRows = 16;
 constexpr int kConsumers = 4;
 constexpr int kThreads = (kConsumers + 1) * 32;
 constexpr int kSpan = 64;  // elements of a 128-byte swizzle span
-// Bits that a row's weights are taken higher by, so that small ones stay in the type's range; taken off where the
-// warps' parts are joined.  2^14 is fp16's highest power but one.
+// Bits that the weights of a row with the (scaled) maximum ms are taken higher by, so that small ones stay in fp16's
+// range; taken off where the warps' parts are joined.  2^14 is the type's highest power but one; past 2^22 the
+// rounding of c m itself moves all weights of a row by a bit and more, and they keep that room.
 template <bool FP16>
-constexpr float kLift = FP16 ? 14.f : 0.f;
+__device__ __forceinline__ float lift_of(float ms) {
+  return FP16 && fabsf(ms) < 4194304.f ? 14.f : 0.f;
+}
 constexpr int kExtra = 2;  // units' time that a tile's start and end take (2,600 cycles, a unit 1,450)
 
 template <int D>
@@ -306,8 +309,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_rows_kernel(const __grid_c
           for (int i = 0; i < NK / 8; ++i) mx = fmaxf(mx, fmaxf(x[i][2 * j], x[i][2 * j + 1]));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          ms[j] = mx == -INFINITY ? 0.f : mx * a.scale_log2 - kLift<FP16>;
-          const float keep = m[j] == -INFINITY ? 0.f : exp2_approx(m[j] * a.scale_log2 - kLift<FP16> - ms[j]);
+          const float top = mx * a.scale_log2, old = m[j] * a.scale_log2;
+          ms[j] = mx == -INFINITY ? 0.f : top - lift_of<FP16>(top);
+          const float keep = m[j] == -INFINITY ? 0.f : exp2_approx(old - lift_of<FP16>(old) - ms[j]);
           if (mx != m[j]) {
             l[j] *= keep;
             if (m[j] != -INFINITY) {
@@ -366,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_rows_kernel(const __grid_c
       for (int w = 0; w < kConsumers; ++w) {
         const float2 ml = merge_ml[w][row];
         // an empty part has o = l = 0, or, with values that are not finite, what it has to add
-        const float f = ml.x == -INFINITY ? 1.f : exp2_approx((ml.x - mx) * a.scale_log2 - kLift<FP16>);
+        const float f = ml.x == -INFINITY ? 1.f : exp2_approx((ml.x - mx) * a.scale_log2 - lift_of<FP16>(ml.x * a.scale_log2));
         const float4 v = *reinterpret_cast<const float4*>(merge_o + (w * kRows + row) * G_::kPitch + d);
         sum += f * ml.y;
         acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
