@@ -7,6 +7,7 @@ import math
 import pytest
 import torch
 
+import serving_reference as R
 from test_gpu_serving import BF16, FP16, attend, attention_case, check_attention, ints
 from vllm_ascend_kvcompress import _native as N
 from vllm_ascend_kvcompress.methods.triattention import kernels as K
@@ -261,3 +262,28 @@ def test_scores_whose_rounding_is_bits(size, dtype, dim, longest):
     assert (out <= top * (1 + 2 * u + 2.0 ** -18)).all() and (out >= bottom * (1 - 2 * u - 2.0 ** -18)).all()
     assert ((out - want).abs() <= want * (2 * u + 2.0 ** -18 + 4.0 ** s - 1)).all()
     assert (lse.double().cpu() - size).abs().max() <= 8 + size * 2.0 ** -21
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, FP16), (128, BF16), (256, BF16), (256, FP16)])
+@pytest.mark.parametrize("longest", [1, 64])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (70, 5)])
+def test_scattered_values_that_are_not_finite_reach_the_rows_that_see_them(dim, dtype, longest, window, sinks):
+    """Single infinite and NaN values anywhere in the values, beside tails that hold nothing else."""
+    new, lens = [130, 1, 7, 64], [400, 129, 7, 300]
+    c = attention_case(new, lens, 4, 2, dim, dtype)
+    g = torch.Generator().manual_seed(dim + longest)
+    hit = torch.rand(c["vc"].shape, generator=g) < 3e-5
+    c["vc"][hit] = torch.tensor([math.inf, -math.inf, math.nan])[torch.randint(0, 3, (int(hit.sum()),), generator=g)].to(dtype)
+    for r, n in enumerate(lens):
+        if n % 128:
+            c["vc"][c["table"][r, (n - 1) // 128], n % 128:] = math.nan
+    out, lse, ob, lb = R.attention(c["q"], c["kc"], c["vc"], c["table"], c["starts"], c["lens"], dim ** -0.5, window, sinks)
+    got = [x.double().cpu() for x in attend(c, window=window, sinks=sinks, max_query_len=longest)]
+    assert 0 < (~out.isfinite()).sum() < out.numel() / 2
+    assert torch.equal(got[0].isnan(), out.isnan())
+    odd = out.isinf()
+    assert torch.equal(got[0].isinf(), odd) and torch.equal(got[0][odd], out[odd])
+    fine = out.isfinite()
+    # a value that is not finite makes its own dim's bound infinite or NaN: the finite dims' are as they were
+    assert ((got[0] - out).abs() <= ob)[fine].all()
+    assert ((got[1] - lse).abs() <= lb).all()

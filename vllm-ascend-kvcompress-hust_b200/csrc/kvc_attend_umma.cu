@@ -98,7 +98,7 @@ struct Geom {
   // barriers, 8 bytes each: places in their array
   enum Bar : int { kFull = 0, kEmpty = S, kQFull = 2 * S, kQEmpty, kSFull, kPFull = kSFull + 4, kODone = kPFull + 4,
                    kSRead = kODone + 4, kOFree, kDone = kOFree + 2, kRead, kCleared, kBars };
-  static constexpr int kTail = kBars * 8 + kMeta * 4 + 16 + (NT == 1 ? 2048 : 0);
+  static constexpr int kTail = kBars * 8 + kMeta * 4 + 48 + (NT == 1 ? 2048 : 0);
   static constexpr int kSmem = NT * kQ + S * kSlot + kTail;
   static_assert(S >= 5 && kSmem <= 227 * 1024 && kSmem > 116 * 1024, "one CTA per SM: it holds every TMEM column");
   static_assert(S * kSlot >= (kMaxAttendRequests + 1 + kLocateInts) * 4, "the prefix sums lie in the ring");
@@ -198,7 +198,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
   const uint32_t vread = full0 + 8 * G_::kRead, vclear = full0 + 8 * G_::kCleared;  // a block's odd values (two halves)
   volatile uint32_t* meta = reinterpret_cast<uint32_t*>(bars + G_::kBars);  // per unit, from the producer
   uint32_t* tmem_slot = const_cast<uint32_t*>(meta + kMeta);
-  float* xch = reinterpret_cast<float*>(tmem_slot + 4);  // [2][2][128] (NT == 1)
+  uint32_t* odd_keys = tmem_slot + 4;  // [warpgroup][4] keys of a block that hold infinite or NaN values, a bit each
+  float* xch = reinterpret_cast<float*>(tmem_slot + 12);  // [2][2][128] (NT == 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if ((q0 & 1023u) != 0) {  // the swizzle goes by the address
@@ -225,6 +226,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
     mbar_init(done, 2);
     mbar_init(vread, 8);
     mbar_init(vclear, 8);
+    for (int i = 0; i < 8; ++i) odd_keys[i] = 0;
     mbar_init_fence();
   }
   if (warp == kMma) {
@@ -515,6 +517,10 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
               // A masked key weighs nothing whatever its value row holds, but 0 * inf
               // is not 0 in the product: infinite and NaN values leave the block
               // here and reach the rows that do see them by addition at the end.
+              // Only the keys that hold some are gone through: NaN past every length
+              // (pages that were never written) costs 12 chunks of 300 tokens 3 to 4 %,
+              // where a walk through the block's keys took 2.5 (head_dim 128) and 4 (256)
+              // times the whole call.  A key that rows do see costs each of them its dims.
               const uint32_t vs = HV * G_::v_at(ga, units);
               if (NT == 1 && g > 0) wait_o(g, 0);  // its V has been in the slots before this one's
 #pragma unroll
@@ -525,10 +531,15 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
               // Each warpgroup looks for itself (with one half they share the block), and nothing is cleared
               // before both have looked, so both find the same.
               constexpr int kLook = NT == 1 ? 256 : 128;
+              uint32_t* keys = odd_keys + (NT == 1 ? 0 : 4 * wg);
               for (int i = tid % kLook; i < kVec; i += kLook) {
                 uint32_t w[4];
                 lds128(vaddr(i), w);
-                odd |= odd_pair<FP16>(w[0]) | odd_pair<FP16>(w[1]) | odd_pair<FP16>(w[2]) | odd_pair<FP16>(w[3]);
+                if (odd_pair<FP16>(w[0]) | odd_pair<FP16>(w[1]) | odd_pair<FP16>(w[2]) | odd_pair<FP16>(w[3])) {
+                  odd = true;
+                  const int key = i / (SK * D / 8) * SK + i % (SK * 8) / 8;  // rows of a box are 8 vectors
+                  atomicOr(keys + key / 32, 1u << (key % 32));
+                }
               }
               const int team = NT == 1 || halves == 2 ? 256 : 128;
               auto meet = [&](uint32_t bar) {  // the team's warps; two halves' by mbarrier
@@ -544,27 +555,30 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
               };
               if (named_or(kBarLook + (NT == 1 ? 0 : wg), kLook, odd)) {
                 const int d0 = NT == 1 ? wg * OC : 0;
-                if (live && !poison) {
-                  for (int d = 0; d < OC; ++d) mine[d] = 0.f;
-                  poison = true;
-                }
-                for (int key = 0; key < KB; ++key) {
-                  if (!live || !attend_sees(a, pos, k0 + key)) continue;
-                  const int row = key % SK;
-                  const uint32_t slot = ring0 + ((vs + key / SK) % S) * G_::kSlot;
-                  for (int d = d0; d < d0 + OC; d += 2) {
-                    uint32_t w;
-                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w)
-                                 : "r"(slot + (d / kSpan) * G_::kBox + row * 128 + ((((d % kSpan) / 8) ^ (row & 7)) << 4) +
-                                       (d % 8) * 2)
-                                 : "memory");
-                    if (!odd_pair<FP16>(w)) continue;
-                    const float2 v = unpack2(w, E{});
-                    if (!isfinite(v.x)) mine[d - d0] += v.x;
-                    if (!isfinite(v.y)) mine[d - d0 + 1] += v.y;
+                // the keys that hold some, where a row sees them (past a request's length none does)
+                for (int k = 0; k < KB / 32; ++k)
+                  for (uint32_t left = live ? *reinterpret_cast<volatile uint32_t*>(keys + k) : 0; left; left &= left - 1) {
+                    const int key = 32 * k + __ffs(left) - 1, row = key % SK;
+                    if (!attend_sees(a, pos, k0 + key)) continue;
+                    if (!poison) {
+                      for (int d = 0; d < OC; ++d) mine[d] = 0.f;
+                      poison = true;
+                    }
+                    const uint32_t slot = ring0 + ((vs + key / SK) % S) * G_::kSlot;
+                    for (int d = d0; d < d0 + OC; d += 2) {
+                      uint32_t w;
+                      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w)
+                                   : "r"(slot + (d / kSpan) * G_::kBox + row * 128 + ((((d % kSpan) / 8) ^ (row & 7)) << 4) +
+                                         (d % 8) * 2)
+                                   : "memory");
+                      if (!odd_pair<FP16>(w)) continue;
+                      const float2 v = unpack2(w, E{});
+                      if (!isfinite(v.x)) mine[d - d0] += v.x;
+                      if (!isfinite(v.y)) mine[d - d0 + 1] += v.y;
+                    }
                   }
-                }
                 meet(vread);  // read by all before it is cleared
+                if (tid % kLook < KB / 32) keys[tid % kLook] = 0;
                 for (int i = team == 256 ? tid : r; i < kVec; i += team) {
                   const uint32_t ad = vaddr(i);
                   uint32_t w[4];
