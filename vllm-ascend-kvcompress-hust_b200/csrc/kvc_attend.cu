@@ -261,19 +261,25 @@ __global__ void __launch_bounds__(kThreads, 1) attend_rows_kernel(const __grid_c
           // A masked key weighs nothing whatever its value row holds, but 0 * inf
           // is not 0 in the product: infinite and NaN values leave the tile here
           // and reach the rows that do see them by addition.
-          uint32_t odd = 0;  // keys that hold some, a bit each
-          static_assert(NK <= 32, "");
+          bool odd = false;
           for (int i = lane; i < NK * (D / 8); i += 32) {
             uint32_t w[4];
             const uint32_t ad = tile_addr<KB>(vt, w0 + i / (D / 8), (i % (D / 8)) * 8);
             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                          : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(ad) : "memory");
-            if (odd_pair<FP16>(w[0]) | odd_pair<FP16>(w[1]) | odd_pair<FP16>(w[2]) | odd_pair<FP16>(w[3]))
-              odd |= 1u << (i / (D / 8));
+            odd |= odd_pair<FP16>(w[0]) | odd_pair<FP16>(w[1]) | odd_pair<FP16>(w[2]) | odd_pair<FP16>(w[3]);
           }
-          odd = __reduce_or_sync(0xffffffffu, odd);
-          if (odd) {
-            for (uint32_t left = odd; left; left &= left - 1) {
+          if (__any_sync(0xffffffffu, odd)) {
+            uint32_t keys = 0;  // that hold some, a bit each
+            static_assert(NK <= 32, "");
+            for (int i = lane; i < NK * (D / 2); i += 32) {
+              uint32_t w;
+              asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w)
+                           : "r"(tile_addr<KB>(vt, w0 + i / (D / 2), (i % (D / 2)) * 2)) : "memory");
+              if (odd_pair<FP16>(w)) keys |= 1u << (i / (D / 2));
+            }
+            keys = __reduce_or_sync(0xffffffffu, keys);
+            for (uint32_t left = keys; left; left &= left - 1) {
               const int key = __ffs(left) - 1;
               const bool sees0 = attend_sees(a, pos[0], k0 + w0 + key), sees1 = attend_sees(a, pos[1], k0 + w0 + key);
               if (!__any_sync(0xffffffffu, sees0 || sees1)) continue;  // past a request's length no row sees it

@@ -531,15 +531,10 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
               // Each warpgroup looks for itself (with one half they share the block), and nothing is cleared
               // before both have looked, so both find the same.
               constexpr int kLook = NT == 1 ? 256 : 128;
-              uint32_t* keys = odd_keys + (NT == 1 ? 0 : 4 * wg);
               for (int i = tid % kLook; i < kVec; i += kLook) {
                 uint32_t w[4];
                 lds128(vaddr(i), w);
-                if (odd_pair<FP16>(w[0]) | odd_pair<FP16>(w[1]) | odd_pair<FP16>(w[2]) | odd_pair<FP16>(w[3])) {
-                  odd = true;
-                  const int key = i / (SK * D / 8) * SK + i % (SK * 8) / 8;  // rows of a box are 8 vectors
-                  atomicOr(keys + key / 32, 1u << (key % 32));
-                }
+                odd |= odd_pair<FP16>(w[0]) | odd_pair<FP16>(w[1]) | odd_pair<FP16>(w[2]) | odd_pair<FP16>(w[3]);
               }
               const int team = NT == 1 || halves == 2 ? 256 : 128;
               auto meet = [&](uint32_t bar) {  // the team's warps; two halves' by mbarrier
@@ -555,6 +550,15 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
               };
               if (named_or(kBarLook + (NT == 1 ? 0 : wg), kLook, odd)) {
                 const int d0 = NT == 1 ? wg * OC : 0;
+                uint32_t* keys = odd_keys + (NT == 1 ? 0 : 4 * wg);
+                for (int i = tid % kLook; odd && i < kVec; i += kLook) {
+                  uint32_t w[4];
+                  lds128(vaddr(i), w);
+                  const int key = i / (SK * D / 8) * SK + i % (SK * 8) / 8;  // rows of a box are 8 vectors
+                  if (odd_pair<FP16>(w[0]) | odd_pair<FP16>(w[1]) | odd_pair<FP16>(w[2]) | odd_pair<FP16>(w[3]))
+                    atomicOr(keys + key / 32, 1u << (key % 32));
+                }
+                named_sync(kBarLook + (NT == 1 ? 0 : wg), kLook);
                 // the keys that hold some, where a row sees them (past a request's length none does)
                 for (int k = 0; k < KB / 32; ++k)
                   for (uint32_t left = live ? *reinterpret_cast<volatile uint32_t*>(keys + k) : 0; left; left &= left - 1) {
