@@ -429,7 +429,9 @@ int kvc_step_tables(const void* computed, int computed_bytes, const void* schedu
  * v [num_tokens][kv_heads][head_dim] to slot slot_mapping[t] of the caches
  * ([num_blocks][128][kv_heads][head_dim], any block stride); a negative slot
  * writes no key or value, one past the cache raises KVC_DEV_TOKEN_RANGE and
- * writes none.  Of two tokens with the same slot either may stay.  All strides
+ * writes none.  Slots have to differ: where two tokens name one, what stays is
+ * made of 16-byte pieces of either.  q_out may be no part of k, v or the caches.
+ * All strides
  * are in elements, multiples of 8; pointers 16-byte aligned; head_dim a
  * multiple of 8, rotary_dim of 16 and at most 256.  axis_of_frequency may be
  * NULL with one axis (up to 8); an entry outside [0, axes) raises
@@ -456,7 +458,8 @@ int kvc_rotary_write(const void* q, int64_t q_token_stride, int64_t q_head_strid
  *   out = sum_i softmax_i(scale * q.k_i) v_i ; lse = log(sum_i exp(scale * q.k_i))
  * A row that sees no key (p < 0) gets 0 and -inf.  Keys and values that a row
  * does not see have no part in it, infinite and NaN ones included.  Rows of q
- * that no request owns are left as they were.  lse [num_tokens][heads] may be NULL.
+ * that no request owns are left as they were, in out and in lse.  lse
+ * [num_tokens][heads] may be NULL.  out may be no part of the inputs.
  * max_query_len bounds the n; it picks the kernel, not the result, except that 0
  * says that no request has new tokens: nothing is launched.
  * Geometries: head_dim 64, 128 or 256, heads / kv_heads <= 16, up to 8192

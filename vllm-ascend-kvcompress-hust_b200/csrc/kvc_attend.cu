@@ -10,10 +10,10 @@
 // warp waits for another inside a tile, and a line of units cut evenly over the
 // SMs, so a batch of unlike lengths ends everywhere at once.
 //
-// Measured: 16 decodes at 8k-52k keys, 16 / 2 heads of 256, 1.15 GB: 180 us, 0.97 of
-// the copy rate; 32 at 4,608, 40 / 8 of 128, 0.61 GB: 103 us, 0.91; 4 decodes of
-// 1k-6k: 16 us on the device, 2 of them to find the CTA's piece, 2 to the first
-// block, 3 to join the parts.
+// Measured on the device, call behind call: 16 decodes at 8k-52k keys, 16 / 2 heads
+// of 256, 1.15 GB: 171 us, the copy rate (175 us); 32 at 4,608, 40 / 8 of 128, 0.61
+// GB: 101 us, 0.92 of it; 4 decodes of 1k-6k: 12.5 us, 2 of them to find the CTA's
+// piece, 2 to the first block, 3 to join the parts.
 //
 // A consumer warp holds the tile's queries, its running maximum, sum and
 // output in registers: S = Q K^T by mma.sync (K by ldmatrix from the swizzled

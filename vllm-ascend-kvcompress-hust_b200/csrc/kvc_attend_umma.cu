@@ -2,14 +2,20 @@
 // (tcgen05, sm_100a).  kvc_attend.cuh has the mathematics and how work is
 // shared out.
 //
-// Bound: the tensor cores (4 D flops per row and visible key), the SM's
+// Floor: the tensor cores (4 D flops per row and visible key) and the SM's
 // exponential unit beside them (128 keys x 128 rows are 16,384 exponentials at
-// 16 a cycle, 1024 cycles, against 8 D cycles of tensor work) and, in a run of
-// such calls, the 1000 W cap.  2048 new tokens over 16,384 at 40 / 8 heads of 128:
-// 0.82 ms, 890 TFLOP/s, 0.54 of the measured burst rate at 1.45 to 1.65 GHz; the
-// same kernel takes 0.60 to 0.65 ms at 1.9 GHz, and changes that saved a tenth
-// of its cycles (an eighth of the exponentials as polynomials on the FMA pipes)
-// left its time as it was.
+// 16 a cycle, 1024 cycles, against 8 D cycles of tensor work).  Bound: neither.
+// 2048 new tokens over 16,384 at 40 / 8 heads of 128 take 1.2 million cycles in
+// which both are busy half the time (51 %): S in 64-key parts reads 6 KB of shared
+// memory for 32 cycles of products (48), the two halves' products and
+// exponentials wait for each other, and a tile's start and end take 25,000
+// cycles.  0.75 to 0.83 ms, 880 to 970 TFLOP/s, as calls follow each other and the
+// 1000 W cap takes the clock to 1.45 to 1.65 GHz; a library product under that cap
+// keeps 1,397 TFLOP/s, so the cap alone is not the bound, though changes that saved
+// a tenth of the cycles (an eighth of the exponentials as polynomials on the FMA
+// pipes) left the time as it was.  K and V are read through L2 once for each 256
+// (128) rows: 3.3 GB for 118 MB here, 2.3 GB for 180 MB in 12 ragged requests at
+// head_dim 256.
 //
 // Roles of a CTA (one per SM: it holds all 512 TMEM columns):
 //  * producer lane: queries of each tile and K/V blocks of 16 or 32 KB into a
@@ -40,11 +46,12 @@
 // 2^-14, so a weight at the maximum is 2^3 there (2^7 at head_dim 256), and 2^9
 // (2^10) once a block's weights have averaged less than 2^-10.  What rounding takes
 // from weights that are below the range all the same is 2^-15 of the row's sum at
-// most; against a maximum of 1, keys under 2^-25 vanished beside a sum that
-// counts them, which many keys behind one strong first token feel.  Not 2^10 from
-// the start: the running maximum then outgrew the type too often (178 us for 119
-// in a windowed 8,191-token prompt at head_dim 64).  The range costs that case 2 %
-// (117 us without), and up to a sixth where scores are spread over tens of bits.
+// most, and from then on 2^-34 of it a key; against a maximum of 1, keys under 2^-25
+// vanished beside a sum that counts them, which many keys behind one strong first
+// token feel.  Not 2^10 from the start: the running maximum then outgrew the type
+// too often (178 us for 119 in a windowed 8,191-token prompt at head_dim 64).  The
+// range costs that case 2 % (117 us without), and up to a sixth where scores are
+// spread over tens of bits.
 //
 // Every wait is bounded (KVC_DEV_TIMEOUT); a softmax warp whose wait ran out
 // goes on without waiting, so every named barrier is met, the other roles
@@ -93,7 +100,8 @@ struct Geom {
   static constexpr int OC = NT == 2 ? D : D / 2;   // O columns of a softmax thread
   // Room of a tile on the line beside its units: cycles of its start and end (first loads, output) over those
   // of a unit, 24,000 / 2,900, 25,000 / 3,900 and 7,000 / 3,400.  Against none: 12 ragged requests at 16 / 2 heads
-  // of 256 295 -> 274 us, an 8,191-token windowed prompt at 16 / 8 of 64 122 -> 115 us; doubled, 278 and 117.
+  // of 256 295 -> 274 us, an 8,191-token windowed prompt at 16 / 8 of 64 122 -> 115 us; doubled, 278 and 117 (the
+  // prompt is 119 now that fp16 weights are taken higher).
   static constexpr int kExtra = D == 256 ? 8 : D == 128 ? 6 : 2;
   // barriers, 8 bytes each: places in their array
   enum Bar : int { kFull = 0, kEmpty = S, kQFull = 2 * S, kQEmpty, kSFull, kPFull = kSFull + 4, kODone = kPFull + 4,
@@ -518,8 +526,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_umma_kernel(const __grid_c
               // is not 0 in the product: infinite and NaN values leave the block
               // here and reach the rows that do see them by addition at the end.
               // Only the keys that hold some are gone through: NaN past every length
-              // (pages that were never written) costs 12 chunks of 300 tokens 3 to 4 %,
-              // where a walk through the block's keys took 2.5 (head_dim 128) and 4 (256)
+              // (pages that were never written) costs 12 chunks of 300 tokens 1 (head_dim
+              // 128) to 9 % (256), where a walk through the block's keys took 2.5 and 4
               // times the whole call.  A key that rows do see costs each of them its dims.
               const uint32_t vs = HV * G_::v_at(ga, units);
               if (NT == 1 && g > 0) wait_o(g, 0);  // its V has been in the slots before this one's

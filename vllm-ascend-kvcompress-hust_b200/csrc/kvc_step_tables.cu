@@ -14,8 +14,8 @@
 // of the R new-token counts in shared memory (R loads that hit L2) instead of
 // a scan kernel before it, and block CTAs need no prefix sum at all.  Larger
 // steps only add CTAs.  Measured: 6 us alone for 4 requests or for 96 with 9,000
-// new tokens and 16 blocks to a page, 3 of them launch; the call from Python is
-// bound by the host (19 us).
+// new tokens and 16 blocks to a page, 3 us behind another kernel; the call from
+// Python is bound by the host (19 us).
 #include <algorithm>
 
 #include "kvc_common.cuh"

@@ -585,7 +585,8 @@ def rotary_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: t
     views of a fused projection included); ``positions`` [N] or [axes, N] int64
     (semantic); ``omega`` [rotary_dim / 2] fp32 with ``axis_of_frequency`` int32
     naming each frequency's axis when there are several; ``slot_mapping`` [N]
-    int64 (physical; negative: nothing is written); caches
+    int64 (physical; negative: nothing is written; no two alike, or their keys
+    and values mix); caches
     ``[blocks, 128, kv_heads, dim]`` with any block stride.  "Half" style pairs,
     as the calibration statistics assume.  Returns the rotated queries
     (``q_out``, which may be ``q``; a new tensor by default).
@@ -650,7 +651,10 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``max_query_len`` is the most new tokens of a request (it picks the kernel;
     a wrong one costs time, not results).  Returns ``out``
     [N, heads, dim], or ``(out, lse)`` with the fp32 logarithm of each row's sum
-    of exponentials.  ``workspace`` (``paged_attention_workspace_bytes``) is
+    of exponentials.  Rows of ``q`` that no request owns (padding of a captured
+    step) are not written: in a new ``out`` and in ``lse`` they hold whatever the
+    memory held, NaN included, so what follows must not mix rows, or an ``out``
+    that was zeroed once is passed in.  ``workspace`` (``paged_attention_workspace_bytes``) is
     allocated per call unless given; one given must not serve two calls that
     run at the same time.
     """
