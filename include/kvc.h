@@ -403,11 +403,10 @@ int kvc_stage_commit(const int64_t* dst_blocks, const int64_t* dst_block_off, in
  * last token get position 0, slot -1 and request -1.  computed, scheduled and
  * page_table hold 4- or 8-byte integers (*_bytes).  A page that the table lacks
  * (past page_width, negative, or whose blocks pass an int32 or slots an int64)
- * raises KVC_DEV_BLOCK_RANGE and gives -1; a
- * negative count, length or physical position, or more new tokens than
- * num_tokens, raises KVC_DEV_TOKEN_RANGE; more blocks than max_blocks raise
- * KVC_DEV_BLOCK_RANGE (max_blocks 0: no block table is wanted, and none is looked
- * at).  Up to 8192 requests.  No table may share memory with another or with an
+ * raises KVC_DEV_BLOCK_RANGE and gives -1; a negative count, length or physical
+ * position, or more new tokens than num_tokens, raises KVC_DEV_TOKEN_RANGE; more
+ * blocks than max_blocks raise KVC_DEV_BLOCK_RANGE (max_blocks 0: no block table
+ * is wanted, and none is looked at).  Up to 8192 requests.  No table may share memory with another or with an
  * input (KVC_EINVAL): lengths of an earlier call are copied before they become
  * this one's, or its tables written to a second set.
  */
@@ -431,9 +430,8 @@ int kvc_step_tables(const void* computed, int computed_bytes, const void* schedu
  * writes no key or value, one past the cache raises KVC_DEV_TOKEN_RANGE and
  * writes none.  Slots have to differ: where two tokens name one, what stays is
  * made of 16-byte pieces of either.  q_out may be no part of k, v or the caches.
- * All strides
- * are in elements, multiples of 8; pointers 16-byte aligned; head_dim a
- * multiple of 8, rotary_dim of 16 and at most 256.  axis_of_frequency may be
+ * All strides are in elements, multiples of 8; pointers 16-byte aligned; head_dim
+ * a multiple of 8, rotary_dim of 16 and at most 256.  axis_of_frequency may be
  * NULL with one axis (up to 8); an entry outside [0, axes) raises
  * KVC_DEV_INDEX_RANGE and counts as 0.
  */
